@@ -36,6 +36,9 @@ typedef enum lfs_status {
     LFS_EUNSUPPORTED = -4
 } lfs_status;
 
+/* Element types of the operators that take more than float32. */
+typedef enum lfs_dtype { LFS_F32 = 0, LFS_BF16 = 1, LFS_F16 = 2 } lfs_dtype;
+
 /* gsplat/Common.h:46-51 */
 typedef enum lfs_camera_model { LFS_PINHOLE = 0, LFS_ORTHO = 1, LFS_FISHEYE = 2, LFS_EQUIRECTANGULAR = 3 } lfs_camera_model;
 
@@ -412,6 +415,66 @@ typedef struct lfs_adam_segment {
  * kernels that run next to this one on other streams. */
 int lfs_adam_step_segments(int n_segments, const lfs_adam_segment* segments /* host */, double beta1, double beta2,
                            double eps, int64_t step_count, float grad_scale, int ctas_per_sm, void* stream);
+
+/* AdamW (Adam with decoupled weight decay) over any number of contiguous tensors, one launch per 384 of them (no counterpart
+ * in the reference, whose optimizer has no weight decay and keeps 32-bit moments): what is trained next to the Gaussians (per-image
+ * codes, exposure matrices, bilateral grids, palettes, small networks) and scenes whose moments should take a quarter of
+ * the memory. With g = grad_scale * grad, t = step_count >= 1:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * Parameters are float32; gradients float32, bfloat16 or float16 (grad_dtype), computed with in 32 bits.
+ * Moments: float32 [n] with both scale pointers NULL, or 8-bit codes [n] with one float32 scale per LFS_ADAMW_BLOCK elements
+ * ([ceil(n / LFS_ADAMW_BLOCK)] each): exp_avg as e4m3, exp_avg_sq as e5m2, value = code * scale, scale = largest magnitude of the block
+ * over the largest code (448, 57344). What is written back is rounded down or up by a threshold that depends on the element's
+ * index and t only, so that a moment that changes by less than the distance of two codes still moves by the right amount over
+ * the steps, and a run repeats bit for bit; a second moment above zero is not held as zero. The update itself uses the moments before
+ * that rounding. A block whose largest magnitude is below 2^-110 is held as zeros; a first moment that is not finite is held as NaN.
+ * All zeros (codes and scales) is a fresh state. Tensors must not overlap. Empty tensors (n = 0) are skipped. Pointers are aligned to their element;
+ * rows of 16 bytes (4 for codes, 8 for 16-bit gradients) let whole vectors be read.
+ * A captured launch repeats its own t when it is replayed. */
+#define LFS_ADAMW_BLOCK 128
+typedef struct lfs_adamw_tensor {
+    float* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;      /* NULL, NULL: 32-bit moments */
+    float* exp_avg_sq_scale;
+    int64_t n;
+    float lr;
+    float weight_decay;
+    int32_t grad_dtype;        /* lfs_dtype */
+    int32_t reserved;
+} lfs_adamw_tensor;
+int lfs_adamw_step_tensors(int n_tensors, const lfs_adamw_tensor* tensors /* host */, double beta1, double beta2, double eps,
+                           int64_t step_count, float grad_scale, void* stream);
+
+/* Moments between their two forms, rounded to the nearest code: second_moment 0 = e4m3, else e5m2 (values >= 0).
+ * codes [n], scales [ceil(n / LFS_ADAMW_BLOCK)]. */
+int lfs_adamw_state_encode(int64_t n, const float* values, int second_moment, uint8_t* codes, float* scales, void* stream);
+int lfs_adamw_state_decode(int64_t n, const uint8_t* codes, const float* scales, int second_moment, float* values, void* stream);
+
+/* Embedding lookup with scaling (no counterpart in the reference): out [n,width] = scale * table [rows,width] at indices [n] (int32 or
+ * int64 by index_bits). An index below 0 or not below `rows` gives a row of zeros. The table is float32, bfloat16 or float16;
+ * out has its type or float32. For tables that many Gaussians or images share: a palette of SH rows, per-image or per-camera codes. */
+#define LFS_EMBEDDING_MAX_WIDTH (1 << 20)
+int lfs_embedding_fwd(int64_t n, int64_t rows, int width, const void* table, int table_dtype, const void* indices, int index_bits,
+                      float scale, void* out, int out_dtype, void* stream);
+
+/* The lookups in the order of their rows, ties by their position: sorted_rows [n] = the rows in ascending order (`rows` for
+ * indices that name none), order [n] = their positions in `indices`. It can be kept for as long as the indices stay the same. n, rows < 2^31 - 1. */
+size_t lfs_embedding_sort_workspace_bytes(int64_t n, int64_t rows);
+int lfs_embedding_sort(int64_t n, int64_t rows, const void* indices, int index_bits, int32_t* order, int32_t* sorted_rows,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradient of lfs_embedding_fwd with respect to the table: v_table [rows,width] float32 = scale * sum over the lookups i of a row of
+ * v_out[i] (v_out [n,width] of type `dtype`), zeros for rows without lookups; added to v_table with `accumulate`. order and sorted_rows are those of
+ * lfs_embedding_sort for the same n and rows. Sums are held in 32 bits and added in the order of the lookups' positions, in chunks
+ * of fixed length: the result does not change from call to call. */
+size_t lfs_embedding_bwd_workspace_bytes(int64_t n, int width);
+int lfs_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order,
+                      const int32_t* sorted_rows, float scale, int accumulate, float* v_table, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* Data-parallel exchange fused with the optimizer (no counterpart in the reference, which is single-GPU):
  * ONE kernel that, for this rank's shard of the flat parameter buffer, loads the gradient of every rank

@@ -11,6 +11,9 @@ LIB_PATH = _HERE / "liblfs_b200.so"
 
 LFS_OK, LFS_EINVAL, LFS_ECAPACITY, LFS_ECUDA, LFS_EUNSUPPORTED = 0, -1, -2, -3, -4
 PINHOLE, ORTHO, FISHEYE, EQUIRECTANGULAR = 0, 1, 2, 3
+LFS_F32, LFS_BF16, LFS_F16 = 0, 1, 2
+LFS_ADAMW_BLOCK = 128
+LFS_EMBEDDING_MAX_WIDTH = 1 << 20
 LFS_DP_MAX_WORLD, LFS_DP_FLAG_SLOTS = 16, 8
 LFS_DP_FLAG_WORDS = LFS_DP_MAX_WORLD * LFS_DP_FLAG_SLOTS
 
@@ -56,6 +59,12 @@ class RenderView(C.Structure):
 class AdamSegment(C.Structure):
     _fields_ = [("param", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("grad", C.c_void_p),
                 ("n", C.c_int64), ("lr", C.c_float)]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p), ("n", C.c_int64), ("lr", C.c_float),
+                ("weight_decay", C.c_float), ("grad_dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
 class DpSegment(C.Structure):
@@ -111,6 +120,12 @@ _SIGNATURES = {
                                       vp, sz, vp],
     "lfs_regularization": [i32, vp, vp, f32, f32, vp, vp, vp, vp],
     "lfs_adam_step_segments": [i32, C.POINTER(AdamSegment), C.c_double, C.c_double, C.c_double, i64, f32, i32, vp],
+    "lfs_adamw_step_tensors": [i32, vp, C.c_double, C.c_double, C.c_double, i64, f32, vp],
+    "lfs_adamw_state_encode": [i64, vp, i32, vp, vp, vp],
+    "lfs_adamw_state_decode": [i64, vp, vp, i32, vp, vp],
+    "lfs_embedding_fwd": [i64, i64, i32, vp, i32, vp, i32, f32, vp, i32, vp],
+    "lfs_embedding_sort": [i64, i64, vp, i32, vp, vp, vp, sz, vp],
+    "lfs_embedding_bwd": [i64, i64, i32, vp, i32, vp, vp, f32, i32, vp, vp, sz, vp],
     "lfs_dp_reduce_adam_broadcast": [i32, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), vp, i32, C.POINTER(DpSegment), C.c_double,
                                      C.c_double, C.c_double, i64, f32, i32, vp],
     "lfs_dp_signal": [i32, C.POINTER(C.c_void_p), i32, i32, i32, vp],
@@ -131,6 +146,8 @@ _SIZE_FUNCS = {
     "lfs_ewa_workspace_bytes": [C.POINTER(EwaConfig)],
     "lfs_photometric_loss_workspace_bytes": [i32, i32],
     "lfs_mcmc_workspace_bytes": [i32],
+    "lfs_embedding_sort_workspace_bytes": [i64, i64],
+    "lfs_embedding_bwd_workspace_bytes": [i64, i32],
 }
 EXPORTED = sorted(list(_SIGNATURES) + list(_SIZE_FUNCS) + ["lfs_last_error", "lfs_build_info", "lfs_profile_enable",
                                                           "lfs_profile_collect"])

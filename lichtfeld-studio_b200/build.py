@@ -24,6 +24,8 @@ SOURCES = [
     ("raster.cu", []),
     ("loss.cu", []),
     ("elementwise.cu", []),
+    ("optim.cu", []),
+    ("embedding.cu", []),
     ("api.cu", []),
     ("noalloc.cu", []),
     ("error.cu", []),

@@ -5,7 +5,9 @@
 #include <cstring>
 
 #include "elementwise.cuh"
+#include "embedding.cuh"
 #include "loss.cuh"
+#include "optim.cuh"
 #include "projection.cuh"
 #include "raster.cuh"
 #include "ewa.cuh"
@@ -1006,6 +1008,102 @@ int lfs_mcmc_apply(int N, int K, int n_sampled, const int64_t* sampled, const in
     LFS_REQUIRE(sampled && new_opacities && new_scales && params, "null pointer");
     return launch_mcmc_apply(N, K, n_sampled, sampled, dst_indices, new_opacities, new_scales, min_opacity, *params, exp_avg,
                              exp_avg_sq, S(stream));
+}
+
+// ---------------------------------------------------------------------------------------------
+static bool dtype_ok(int dtype) { return dtype == LFS_F32 || dtype == LFS_BF16 || dtype == LFS_F16; }
+
+int lfs_adamw_step_tensors(int n_tensors, const lfs_adamw_tensor* tensors, double beta1, double beta2, double eps, int64_t step_count, float grad_scale,
+                           void* stream) {
+    LFS_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || tensors), "bad tensor list");
+    LFS_REQUIRE(step_count >= 1, "step_count must be >= 1");
+    LFS_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "betas must be in [0, 1)");
+    LFS_REQUIRE(eps >= 0.0, "eps must not be negative");
+    for (int k = 0; k < n_tensors; ++k) {
+        const lfs_adamw_tensor& t = tensors[k];
+        LFS_REQUIRE(t.n >= 0 && t.n < (int64_t)1 << 37, "bad size");
+        if (t.n == 0) continue;
+        LFS_REQUIRE(t.param && t.grad && t.exp_avg && t.exp_avg_sq, "null pointer in a tensor");
+        LFS_REQUIRE(dtype_ok(t.grad_dtype), "grad_dtype must be LFS_F32, LFS_BF16 or LFS_F16");
+        LFS_REQUIRE((t.exp_avg_scale == nullptr) == (t.exp_avg_sq_scale == nullptr), "both moments are held in 8 bits (two scale arrays) or both in 32 (none)");
+        LFS_REQUIRE(aligned_by(t.param, 4) && aligned_by(t.grad, dtype_bytes(t.grad_dtype)) && aligned_by(t.exp_avg_scale, 4) && aligned_by(t.exp_avg_sq_scale, 4),
+                    "misaligned pointer");
+        LFS_REQUIRE(t.exp_avg_scale || (aligned_by(t.exp_avg, 4) && aligned_by(t.exp_avg_sq, 4)), "misaligned pointer");
+    }
+    return launch_adamw_tensors(n_tensors, tensors, beta1, beta2, eps, step_count, grad_scale, S(stream));
+}
+
+int lfs_adamw_state_encode(int64_t n, const float* values, int second_moment, uint8_t* codes, float* scales, void* stream) {
+    LFS_REQUIRE(n >= 0 && n < (int64_t)1 << 37, "bad size");
+    if (n == 0) return LFS_OK;
+    LFS_REQUIRE(values && codes && scales, "null pointer");
+    LFS_REQUIRE(aligned_by(values, 4) && aligned_by(scales, 4), "misaligned pointer");
+    return launch_adamw_encode(n, values, second_moment, codes, scales, S(stream));
+}
+
+int lfs_adamw_state_decode(int64_t n, const uint8_t* codes, const float* scales, int second_moment, float* values, void* stream) {
+    LFS_REQUIRE(n >= 0 && n < (int64_t)1 << 37, "bad size");
+    if (n == 0) return LFS_OK;
+    LFS_REQUIRE(values && codes && scales, "null pointer");
+    LFS_REQUIRE(aligned_by(values, 4) && aligned_by(scales, 4), "misaligned pointer");
+    return launch_adamw_decode(n, codes, scales, second_moment, values, S(stream));
+}
+
+// ---------------------------------------------------------------------------------------------
+static int check_embedding(const char* who, int64_t n, int64_t rows, int width) {
+    if (n < 0 || n >= ((int64_t)1 << 31) - 1 || rows < 1 || rows >= ((int64_t)1 << 31) - 1 || width < 1 || width > LFS_EMBEDDING_MAX_WIDTH) {
+        set_error("%s: bad sizes", who);
+        return LFS_EINVAL;
+    }
+    return LFS_OK;
+}
+
+int lfs_embedding_fwd(int64_t n, int64_t rows, int width, const void* table, int table_dtype, const void* indices, int index_bits, float scale, void* out,
+                      int out_dtype, void* stream) {
+    const int rc = check_embedding("lfs_embedding_fwd", n, rows, width);
+    if (rc != LFS_OK) return rc;
+    LFS_REQUIRE(dtype_ok(table_dtype) && (out_dtype == table_dtype || out_dtype == LFS_F32), "out_dtype must be table_dtype or LFS_F32");
+    LFS_REQUIRE(index_bits == 32 || index_bits == 64, "index_bits must be 32 or 64");
+    if (n == 0) return LFS_OK;
+    LFS_REQUIRE(table && indices && out, "null pointer");
+    LFS_REQUIRE(aligned_by(table, dtype_bytes(table_dtype)) && aligned_by(out, dtype_bytes(out_dtype)) && aligned_by(indices, (uintptr_t)index_bits / 8), "misaligned pointer");
+    return launch_embedding_fwd(n, rows, width, table, table_dtype, indices, index_bits, scale, out, out_dtype, S(stream));
+}
+
+size_t lfs_embedding_sort_workspace_bytes(int64_t n, int64_t rows) {
+    if (check_embedding("lfs_embedding_sort_workspace_bytes", n, rows, 1) != LFS_OK) return 0;
+    return embedding_sort_bytes(n, rows);
+}
+
+int lfs_embedding_sort(int64_t n, int64_t rows, const void* indices, int index_bits, int32_t* order, int32_t* sorted_rows, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    const int rc = check_embedding("lfs_embedding_sort", n, rows, 1);
+    if (rc != LFS_OK) return rc;
+    LFS_REQUIRE(index_bits == 32 || index_bits == 64, "index_bits must be 32 or 64");
+    if (n == 0) return LFS_OK;
+    LFS_REQUIRE(indices && order && sorted_rows && workspace, "null pointer");
+    LFS_REQUIRE(aligned_by(indices, (uintptr_t)index_bits / 8) && aligned_by(order, 4) && aligned_by(sorted_rows, 4) && aligned_by(workspace, 256), "misaligned pointer");
+    if (workspace_bytes < embedding_sort_bytes(n, rows)) { set_error("lfs_embedding_sort: workspace too small"); return LFS_ECAPACITY; }
+    return launch_embedding_sort(n, rows, indices, index_bits, order, sorted_rows, workspace, S(stream));
+}
+
+size_t lfs_embedding_bwd_workspace_bytes(int64_t n, int width) {
+    if (check_embedding("lfs_embedding_bwd_workspace_bytes", n, 1, width) != LFS_OK) return 0;
+    return embedding_bwd_bytes(n, width);
+}
+
+int lfs_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, float scale,
+                      int accumulate, float* v_table, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check_embedding("lfs_embedding_bwd", n, rows, width);
+    if (rc != LFS_OK) return rc;
+    LFS_REQUIRE(dtype_ok(dtype), "dtype must be LFS_F32, LFS_BF16 or LFS_F16");
+    LFS_REQUIRE(v_table && aligned_by(v_table, 4), "null or misaligned v_table");
+    if (n > 0) {
+        LFS_REQUIRE(v_out && order && sorted_rows && workspace, "null pointer");
+        LFS_REQUIRE(aligned_by(v_out, dtype_bytes(dtype)) && aligned_by(order, 4) && aligned_by(sorted_rows, 4) && aligned_by(workspace, 256), "misaligned pointer");
+        if (workspace_bytes < embedding_bwd_bytes(n, width)) { set_error("lfs_embedding_bwd: workspace too small"); return LFS_ECAPACITY; }
+    }
+    return launch_embedding_bwd(n, rows, width, v_out, dtype, order, sorted_rows, scale, accumulate, v_table, workspace, S(stream));
 }
 
 }  // extern "C"

@@ -48,6 +48,9 @@ inline int grid_for(int64_t n, int block, int max_blocks_per_sm = 8) {
     return (int)g;
 }
 
+inline bool aligned_by(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline size_t dtype_bytes(int dtype) { return dtype == LFS_F32 ? 4 : 2; }
+
 template <class... P, class... A>
 void launch(void (*kernel)(P...), int grid, int block, size_t smem, cudaStream_t st, A... args) { kernel<<<grid, block, smem, st>>>(args...); }
 // A launch that starts as soon as every CTA of the launch before it has called let_next_start() or has ended. That launch has to have started behind everything

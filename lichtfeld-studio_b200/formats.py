@@ -8,7 +8,8 @@
 * Checkpoint (no counterpart file format in the reference, which resumes from PLY only): parameters, both Adam
   moments, the step count, learning rates and strategy counters in one flat binary file:
       magic "LFSCKPT1" | uint64 header length | JSON header | float32 payload (params, exp_avg, exp_avg_sq rows)
-  Each payload section is the six groups [means | sh0 | shN | scaling | rotation | opacity] of the LIVE rows."""
+  Each payload section is the six groups [means | sh0 | shN | scaling | rotation | opacity] of the LIVE rows; 8-bit moments
+  (header "state_bits": 8) are stored as they are held, the codes of a group and then its float32 scales."""
 from __future__ import annotations
 
 import ctypes as C
@@ -21,6 +22,7 @@ import torch
 
 from . import _capi as capi
 from ._capi import call, ptr
+from .strategy import PackedMoments
 from .trainer import PARAM_NAMES, SplatData
 
 _MAGIC = b"LFSCKPT1"
@@ -130,6 +132,14 @@ def _sections(strategy):
     return [("params", strategy.get_model()), ("exp_avg", opt.exp_avg), ("exp_avg_sq", opt.exp_avg_sq)]
 
 
+def _live_buffers(sd, name):
+    """The tensors that hold one group's live rows, with the numpy type they are written as."""
+    if isinstance(sd, PackedMoments):
+        codes, scales = sd.live(name)
+        return [(codes.view(torch.uint8), "u1"), (scales, "<f4")]
+    return [(sd.tensor(name), "<f4")]
+
+
 def save_checkpoint(strategy, path: str, iteration: int) -> str:
     """Everything needed to continue training bit-identically: live rows of the parameters and both Adam moments,
     optimizer step count, per-group learning rates (after decay), active SH degree and the iteration."""
@@ -137,7 +147,7 @@ def save_checkpoint(strategy, path: str, iteration: int) -> str:
     n = model.size
     header = dict(version=1, iteration=int(iteration), n=n, sh_coeffs=model.K, step_count=int(opt.step_count), lr=list(opt.lr),
                   betas=list(opt.betas), eps=opt.eps, active_sh_degree=int(getattr(strategy, "active_sh_degree", 0)),
-                  strategy=type(strategy).__name__, sections=[s for s, _ in _sections(strategy)], groups=list(PARAM_NAMES))
+                  strategy=type(strategy).__name__, state_bits=getattr(opt, "state_bits", 32), sections=[s for s, _ in _sections(strategy)], groups=list(PARAM_NAMES))
     hj = json.dumps(header).encode("utf-8")
     tmp = path + ".tmp"
     with open(tmp, "wb") as f:
@@ -147,7 +157,8 @@ def save_checkpoint(strategy, path: str, iteration: int) -> str:
         for _, sd in _sections(strategy):
             sd.size = n
             for name in PARAM_NAMES:
-                f.write(sd.tensor(name).detach().cpu().numpy().astype("<f4", copy=False).tobytes())
+                for t, kind in _live_buffers(sd, name):
+                    f.write(t.detach().cpu().numpy().astype(kind, copy=False).tobytes())
     os.replace(tmp, path)  # a crash while writing never leaves a truncated checkpoint under the final name
     return path
 
@@ -167,14 +178,17 @@ def load_checkpoint(strategy, path: str) -> int:
             raise RuntimeError(f"{path}: {n} Gaussians exceed the model's capacity {model.capacity}")
         if header.get("groups") != list(PARAM_NAMES):
             raise RuntimeError(f"{path}: unexpected group order")
+        if header.get("state_bits", 32) != getattr(opt, "state_bits", 32):
+            raise RuntimeError(f"{path}: moments in {header.get('state_bits', 32)} bits, the optimizer keeps {getattr(opt, 'state_bits', 32)}")
         for _, sd in _sections(strategy):
             sd.size = n
             for name in PARAM_NAMES:
-                t = sd.tensor(name)
-                raw = f.read(t.numel() * 4)
-                if len(raw) != t.numel() * 4:
-                    raise RuntimeError(f"{path}: truncated payload")
-                t.copy_(torch.from_numpy(np.frombuffer(raw, dtype="<f4").copy()).reshape(t.shape))
+                for t, kind in _live_buffers(sd, name):
+                    size = t.numel() * t.element_size()
+                    raw = f.read(size)
+                    if len(raw) != size:
+                        raise RuntimeError(f"{path}: truncated payload")
+                    t.copy_(torch.from_numpy(np.frombuffer(raw, dtype=kind).copy()).reshape(t.shape))
     if hasattr(strategy, "grads"):
         strategy.grads.size = n
     opt.step_count = int(header["step_count"])

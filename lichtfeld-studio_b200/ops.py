@@ -288,6 +288,132 @@ def adam_step_wrapper(param, exp_avg, exp_avg_sq, param_grad, lr, beta1, beta2, 
          float(beta2), float(eps), float(bias_correction1_rcp), float(bias_correction2_sqrt_rcp), _stream())
 
 
+# ---- operators without a counterpart in the reference: embeddings, moments in 8 bits ------------------------------------------
+_DTYPES = {torch.float32: capi.LFS_F32, torch.bfloat16: capi.LFS_BF16, torch.float16: capi.LFS_F16}
+_MAX_ROWS = (1 << 31) - 2
+
+
+def _call_on(device, name, *args):
+    """The call on the current stream of the tensors' device, which becomes the current one for it."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _stream())
+
+
+def _check_typed(t, name, dtypes, device=None):
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name} must be {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, got {t.device}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+
+
+def embedding_fwd(table, indices, scale=1.0, out_dtype=None, out=None):
+    """scale * table[indices]: [*indices.shape, width] of the table's type or float32. table [rows, width] float32, bfloat16 or
+    float16; indices int32 or int64 of any shape. An index below 0 or not below `rows` gives zeros. `out` receives the result
+    (contiguous, its element type is the out_dtype)."""
+    _check_typed(table, "table", _DTYPES)
+    if table.dim() != 2 or not 1 <= table.shape[0] <= _MAX_ROWS or not 1 <= table.shape[1] <= capi.LFS_EMBEDDING_MAX_WIDTH:
+        raise RuntimeError(f"table must be [rows, width] with at least one row and column, got {list(table.shape)}")
+    _check_typed(indices, "indices", (torch.int32, torch.int64), table.device)
+    rows, width = table.shape
+    shape = (*indices.shape, width)
+    if indices.numel() > _MAX_ROWS:
+        raise RuntimeError("too many indices")
+    if out is None:
+        dtype = out_dtype or table.dtype
+    else:
+        dtype = out.dtype
+        if out_dtype not in (None, dtype) or out.numel() != indices.numel() * width:
+            raise RuntimeError(f"out must hold {indices.numel()} rows of {width} elements of the out_dtype")
+        _check_typed(out, "out", _DTYPES, table.device)
+    if dtype not in (table.dtype, torch.float32):
+        raise RuntimeError(f"out must be {table.dtype} or torch.float32, got {dtype}")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=table.device)
+    if indices.numel():
+        _call_on(table.device, "lfs_embedding_fwd", indices.numel(), rows, width, ptr(table), _DTYPES[table.dtype], ptr(indices),
+                 indices.element_size() * 8, float(scale), ptr(out), _DTYPES[dtype])
+    return out
+
+
+class EmbeddingOrder:
+    """The lookups of one tensor of indices in the order of their rows (embedding_sort), for as many embedding_bwd as share it."""
+
+    def __init__(self, shape, rows, order, sorted_rows):
+        self.shape, self.rows, self.order, self.sorted_rows = shape, rows, order, sorted_rows
+
+
+def embedding_sort(indices, rows):
+    """The order that embedding_bwd goes by. Stable: lookups of one row stay in the order of their positions."""
+    _check_typed(indices, "indices", (torch.int32, torch.int64))
+    rows, n, dev = int(rows), indices.numel(), indices.device
+    if not 1 <= rows <= _MAX_ROWS or n > _MAX_ROWS:
+        raise RuntimeError(f"bad sizes: {n} indices, {rows} rows")
+    order, sorted_rows = torch.empty((2, n), dtype=torch.int32, device=dev)
+    if n:
+        ws = _ws(capi.lib().lfs_embedding_sort_workspace_bytes(n, rows), dev)
+        _call_on(dev, "lfs_embedding_sort", n, rows, ptr(indices), indices.element_size() * 8, ptr(order), ptr(sorted_rows), ptr(ws), ws.numel())
+    return EmbeddingOrder(indices.shape, rows, order, sorted_rows)
+
+
+def embedding_bwd(v_out, order, scale=1.0, out=None, accumulate=False):
+    """Gradient of embedding_fwd with respect to the table: [rows, width] float32, scale times the sum of v_out over every row's
+    lookups, zeros for rows without any. v_out [*indices.shape, width] float32, bfloat16 or float16. `out` receives it, or is added to with
+    `accumulate`. The same call gives the same bits."""
+    if not isinstance(order, EmbeddingOrder):
+        raise RuntimeError("order must come from embedding_sort")
+    _check_typed(v_out, "v_out", _DTYPES, order.order.device)
+    n, rows = order.order.numel(), order.rows
+    if v_out.dim() < 1 or v_out.shape[:-1] != order.shape or not 1 <= v_out.shape[-1] <= capi.LFS_EMBEDDING_MAX_WIDTH:
+        raise RuntimeError(f"v_out must be {[*order.shape, 'width']}, got {list(v_out.shape)}")
+    width, dev = v_out.shape[-1], v_out.device
+    if out is None:
+        if accumulate:
+            raise RuntimeError("accumulate needs an out to add to")
+        out = torch.empty((rows, width), dtype=torch.float32, device=dev)
+    else:
+        _check_typed(out, "out", (torch.float32,), dev)
+        if out.numel() != rows * width:
+            raise RuntimeError(f"out must hold {rows} rows of {width} elements")
+    ws = _ws(capi.lib().lfs_embedding_bwd_workspace_bytes(n, width), dev)
+    _call_on(dev, "lfs_embedding_bwd", n, rows, width, ptr(v_out), _DTYPES[v_out.dtype], ptr(order.order), ptr(order.sorted_rows), float(scale),
+             1 if accumulate else 0, ptr(out), ptr(ws), ws.numel())
+    return out
+
+
+def adamw_state_encode(values, second_moment=False):
+    """float32 moments -> (codes of the same shape, float32 scales of their blocks of 128), rounded to the nearest code. The first
+    moment is held as torch.float8_e4m3fn, the second (values >= 0) as torch.float8_e5m2."""
+    _check_typed(values, "values", (torch.float32,))
+    n = values.numel()
+    codes = torch.empty(values.shape, dtype=torch.float8_e5m2 if second_moment else torch.float8_e4m3fn, device=values.device)
+    scales = torch.empty(-(-n // capi.LFS_ADAMW_BLOCK), dtype=torch.float32, device=values.device)
+    if n:
+        _call_on(values.device, "lfs_adamw_state_encode", n, ptr(values), 1 if second_moment else 0, ptr(codes), ptr(scales))
+    return codes, scales
+
+
+def adamw_state_decode(codes, scales):
+    """The float32 values that 8-bit moments stand for."""
+    _check_typed(codes, "codes", (torch.float8_e4m3fn, torch.float8_e5m2))
+    _check_typed(scales, "scales", (torch.float32,), codes.device)
+    n = codes.numel()
+    if scales.numel() != -(-n // capi.LFS_ADAMW_BLOCK):
+        raise RuntimeError(f"{n} codes have {-(-n // capi.LFS_ADAMW_BLOCK)} scales, got {scales.numel()}")
+    values = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+    if n:
+        _call_on(codes.device, "lfs_adamw_state_decode", n, ptr(codes), ptr(scales), 1 if codes.dtype == torch.float8_e5m2 else 0, ptr(values))
+    return values
+
+
 # gsplat/Ops.h:162-270: the fused operator pair, composed from the operator-level entry points with
 # the same torch glue as gsplat/Rasterization.cpp:326-466 / :527-641 (all five render modes, compensations, masks).
 def rasterize_from_world_with_sh_fwd(means, quats, scales, opacities, sh_coeffs, sh_degree, backgrounds, masks, image_width,

@@ -17,9 +17,9 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import _capi as capi
+from . import _capi as capi, ops
 from ._capi import call, ptr
-from .trainer import SplatData, adam_step_splats
+from .trainer import PARAM_NAMES, SplatData, adam_step_splats
 
 
 def _stream():
@@ -44,6 +44,10 @@ class OptimizationParameters:
     max_cap: int = 1_000_000
     sh_degree: int = 3
     scene_scale: float = 1.0
+    # no counterpart in the reference
+    optimizer: str = "adam"                        # "adam" (FusedAdam) or "adamw" (FusedAdamW)
+    weight_decay: float | tuple[float, ...] = 0.0  # adamw: one value, or one per parameter group
+    state_bits: int = 32                           # adamw: moments in 32 or 8 bits
 
 
 class FusedAdam:
@@ -74,6 +78,210 @@ class FusedAdam:
 
     def zero_grad(self, set_to_none=True, iteration=0):
         """No-op: the next backward overwrites every gradient row."""
+
+
+@dataclass
+class Moments:
+    """The moments of one tensor: float32, or 8-bit codes (e4m3, e5m2) with the scales of their blocks of 128 elements."""
+    exp_avg: torch.Tensor
+    exp_avg_sq: torch.Tensor
+    exp_avg_scale: torch.Tensor | None = None
+    exp_avg_sq_scale: torch.Tensor | None = None
+
+    @staticmethod
+    def zeros(n: int, state_bits: int, device) -> "Moments":
+        if state_bits == 32:
+            return Moments(*(torch.zeros(n, dtype=torch.float32, device=device) for _ in range(2)))
+        if state_bits != 8:
+            raise RuntimeError(f"state_bits must be 32 or 8, got {state_bits}")
+        codes = [torch.zeros(n, dtype=torch.uint8, device=device).view(t) for t in (torch.float8_e4m3fn, torch.float8_e5m2)]
+        return Moments(*codes, *(torch.zeros(-(-n // capi.LFS_ADAMW_BLOCK), dtype=torch.float32, device=device) for _ in range(2)))
+
+    def check(self, n: int, device, what: str):
+        bits = 32 if self.exp_avg_scale is None and self.exp_avg_sq_scale is None else 8
+        if bits == 8 and (self.exp_avg_scale is None or self.exp_avg_sq_scale is None):
+            raise RuntimeError(f"{what}: both moments have scales, or neither")
+        types = (torch.float32, torch.float32) if bits == 32 else (torch.float8_e4m3fn, torch.float8_e5m2)
+        for t, name, dtype in zip((self.exp_avg, self.exp_avg_sq), ("exp_avg", "exp_avg_sq"), types):
+            ops._check_typed(t, f"{what}.{name}", (dtype,), device)
+            if t.numel() != n:
+                raise RuntimeError(f"{what}.{name} must have {n} elements, got {t.numel()}")
+        for t, name in zip((self.exp_avg_scale, self.exp_avg_sq_scale), ("exp_avg_scale", "exp_avg_sq_scale")):
+            if bits == 8:
+                ops._check_typed(t, f"{what}.{name}", (torch.float32,), device)
+                if t.numel() != -(-n // capi.LFS_ADAMW_BLOCK):
+                    raise RuntimeError(f"{what}.{name} must have {-(-n // capi.LFS_ADAMW_BLOCK)} elements, got {t.numel()}")
+
+
+_TABLE = np.dtype([("param", "u8"), ("grad", "u8"), ("exp_avg", "u8"), ("exp_avg_sq", "u8"), ("exp_avg_scale", "u8"), ("exp_avg_sq_scale", "u8"),
+                   ("n", "i8"), ("lr", "f4"), ("weight_decay", "f4"), ("grad_dtype", "i4"), ("reserved", "i4")])   # lfs_adamw_tensor
+
+
+def _each(value, n: int, name: str) -> list:
+    """One float per tensor from one for all or a list."""
+    values = [float(value)] * n if isinstance(value, (int, float)) else [float(x) for x in value]
+    if len(values) != n:
+        raise RuntimeError(f"{name}: {len(values)} values for {n} tensors")
+    return values
+
+
+def _check_betas(betas, eps):
+    if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2 or not eps >= 0.0:
+        raise RuntimeError(f"betas must be two numbers in [0, 1) and eps not negative, got {betas}, {eps}")
+
+
+class AdamW:
+    """AdamW over a list of tensors, one launch per 384 of them (lfs_adamw_step_tensors): per-image codes, exposure matrices, grids,
+    palettes, small networks. Parameters are contiguous float32, gradients contiguous float32, bfloat16 or float16 of the same number of elements, on one device.
+
+    Parameters, gradients and moments are bound here and stay bound: a step reads the gradients that are in those buffers by then (torch: zero_grad(set_to_none=False)),
+    and set_grads binds others. None in the place of a gradient leaves its parameter out. `lr` and `weight_decay` (one value or one per tensor) are
+    read at every step, so a scheduler may change them. moments: those of a run to continue; else zeros, in state_bits (32 or 8) bits."""
+
+    def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, moments=None):
+        params = list(params)
+        if not params:
+            raise RuntimeError("AdamW needs at least one tensor")
+        n = len(params)
+        self.betas, self.eps = tuple(float(b) for b in betas), float(eps)
+        _check_betas(self.betas, self.eps)
+        self.device = params[0].device
+        for i, p in enumerate(params):
+            ops._check_typed(p, f"params[{i}]", (torch.float32,), self.device)
+        spans = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise RuntimeError("params must not overlap")
+        self.params = [p.detach() for p in params]   # keeps the memory that the kernel writes to
+        if moments is None:
+            moments = [Moments.zeros(p.numel(), b, self.device) for p, b in zip(self.params, self._bits(state_bits, n))]
+        self.moments = list(moments)
+        if len(self.moments) != n:
+            raise RuntimeError(f"moments: {len(self.moments)} for {n} tensors")
+        for i, (p, m) in enumerate(zip(self.params, self.moments)):
+            m.check(p.numel(), self.device, f"moments[{i}]")
+        self.lr, self.weight_decay = _each(lr, n, "lr"), _each(weight_decay, n, "weight_decay")
+        self.step_count = 0
+        self._table = np.zeros(n, _TABLE)
+        self._table["param"] = [p.data_ptr() for p in self.params]
+        for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+            self._table[name] = [0 if getattr(m, name) is None else getattr(m, name).data_ptr() for m in self.moments]
+        self.set_grads(grads)
+
+    @staticmethod
+    def _bits(state_bits, n):
+        bits = [state_bits] * n if isinstance(state_bits, int) else list(state_bits)
+        if len(bits) != n:
+            raise RuntimeError(f"state_bits: {len(bits)} values for {n} tensors")
+        return bits
+
+    def set_grads(self, grads):
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise RuntimeError(f"grads: {len(grads)} for {len(self.params)} tensors")
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if g is None:
+                continue
+            ops._check_typed(g, f"grads[{i}]", ops._DTYPES, self.device)
+            if g.numel() != p.numel():
+                raise RuntimeError(f"grads[{i}] must have {p.numel()} elements, got {g.numel()}")
+        self.grads = [None if g is None else g.detach() for g in grads]
+        self._table["n"] = [0 if g is None else g.numel() for g in grads]
+        self._table["grad"] = [0 if g is None else g.data_ptr() for g in grads]
+        self._table["grad_dtype"] = [0 if g is None else ops._DTYPES[g.dtype] for g in grads]
+
+    def step(self, grad_scale: float = 1.0):
+        """One update from the bound gradients, which grad_scale multiplies."""
+        self._table["lr"], self._table["weight_decay"] = self.lr, self.weight_decay
+        ops._call_on(self.device, "lfs_adamw_step_tensors", len(self._table), self._table.ctypes.data, self.betas[0], self.betas[1], self.eps,
+                     self.step_count + 1, float(grad_scale))
+        self.step_count += 1
+
+
+class PackedMoments:
+    """One Adam moment of all six groups in 8 bits: what SplatData is for 32-bit moments. tensor() gives the values that the codes of the live rows stand for (a copy),
+    put() encodes new ones. Rows at and above `size` are cleared when they come into use (zero_rows)."""
+
+    def __init__(self, model: SplatData, second: bool):
+        self.capacity, self.size, self.device, self.K, self._w = model.capacity, model.size, model.device, model.K, model._w
+        self.second = second
+        self.codes, self.scales = {}, {}
+        for name in PARAM_NAMES:
+            m = Moments.zeros(self.capacity * self._w[name], 8, self.device)
+            self.codes[name], self.scales[name] = (m.exp_avg_sq, m.exp_avg_sq_scale) if second else (m.exp_avg, m.exp_avg_scale)
+
+    def live(self, name: str):
+        """Codes and scales of the live rows."""
+        n = self.size * self._w[name]
+        return self.codes[name][:n], self.scales[name][:-(-n // capi.LFS_ADAMW_BLOCK)]
+
+    def tensor(self, name: str) -> torch.Tensor:
+        t = ops.adamw_state_decode(*self.live(name))
+        return t.view(self.size, -1, 3) if name in ("sh0", "shN") else t.view(self.size, self._w[name])
+
+    def put(self, name: str, rows: torch.Tensor):
+        codes, scales = self.live(name)
+        c, s = ops.adamw_state_encode(rows.reshape(-1).contiguous(), self.second)
+        codes.view(torch.uint8).copy_(c.view(torch.uint8))
+        scales.copy_(s)
+
+    def zero_rows(self, rows):
+        """rows: an int64 tensor, or a slice."""
+        for name in PARAM_NAMES:
+            if self._w[name] == 0:
+                continue
+            codes = self.codes[name].view(torch.uint8).view(self.capacity, self._w[name])
+            if isinstance(rows, slice):
+                codes[rows] = 0
+            else:
+                codes.index_fill_(0, rows, 0)
+
+
+class FusedAdamW(FusedAdam):
+    """FusedAdam's interface with decoupled weight decay (one value or one per group) and moments in 32 or 8 bits, one launch per step. With 8 bits the
+    moments of a scene take 118 bytes per Gaussian at SH degree 3 instead of 472; exp_avg and exp_avg_sq are PackedMoments."""
+
+    def __init__(self, model: SplatData, lrs, betas=(0.9, 0.999), eps=1e-15, weight_decay=0.0, state_bits: int = 32):
+        if state_bits not in (32, 8):
+            raise RuntimeError(f"state_bits must be 32 or 8, got {state_bits}")
+        _check_betas(betas, eps)
+        self.model = model
+        self.lr = _each(lrs, 6, "lrs")
+        self.weight_decay = _each(weight_decay, 6, "weight_decay")
+        self.betas, self.eps = (float(betas[0]), float(betas[1])), float(eps)
+        self.state_bits = state_bits
+        if state_bits == 32:
+            self.exp_avg, self.exp_avg_sq = model.like(), model.like()
+        else:
+            self.exp_avg, self.exp_avg_sq = PackedMoments(model, False), PackedMoments(model, True)
+        self.step_count = 0
+        self._table = np.zeros(6, _TABLE)
+
+    def step(self, iteration: int, grads: SplatData, grad_scale: float = 1.0, first_row: int = 0, n_rows=None, rasterizer=None):
+        if rasterizer is not None or first_row != 0 or n_rows not in (None, self.model.size):
+            raise RuntimeError("FusedAdamW updates all rows from materialised gradients")
+        self.exp_avg.size = self.exp_avg_sq.size = grads.size = self.model.size
+        packed = self.state_bits == 8
+        for i, name in enumerate(PARAM_NAMES):
+            n = 0 if name == "shN" and iteration <= 1000 else self.model.size * self.model._w[name]   # fused_adam.cpp:66-70
+            moments = [x.codes[name] if packed else x._full[name] for x in (self.exp_avg, self.exp_avg_sq)]
+            scales = [x.scales[name].data_ptr() if packed else 0 for x in (self.exp_avg, self.exp_avg_sq)]
+            self._table[i] = (self.model._full[name].data_ptr(), grads._full[name].data_ptr(), moments[0].data_ptr(), moments[1].data_ptr(), *scales,
+                              n, self.lr[i], self.weight_decay[i], capi.LFS_F32, 0)
+        ops._call_on(self.model.flat.device, "lfs_adamw_step_tensors", 6, self._table.ctypes.data, self.betas[0], self.betas[1], self.eps,
+                     self.step_count + 1, float(grad_scale))
+        self.step_count += 1
+
+
+def make_optimizer(model: SplatData, lrs, params) -> FusedAdam:
+    """The optimizer that OptimizationParameters names."""
+    kind, decay, bits = getattr(params, "optimizer", "adam"), getattr(params, "weight_decay", 0.0), getattr(params, "state_bits", 32)
+    if kind == "adamw":
+        return FusedAdamW(model, lrs, (0.9, 0.999), 1e-15, decay, bits)
+    if kind != "adam":
+        raise RuntimeError(f"optimizer must be adam or adamw, got {kind}")
+    if bits != 32 or (decay if isinstance(decay, (int, float)) else any(decay)):
+        raise RuntimeError("weight_decay and state_bits need optimizer=\"adamw\"")
+    return FusedAdam(model, lrs, (0.9, 0.999), 1e-15)
 
 
 class ExponentialLR:
@@ -132,7 +340,7 @@ class MCMC(IStrategy):
         dev = self._splat_data.device
         self._binoms = torch.from_numpy(binoms_table(51)).to(dev)
         lrs = [p.means_lr * p.scene_scale, p.shs_lr, p.shs_lr / 20.0, p.scaling_lr, p.rotation_lr, p.opacity_lr]  # mcmc.cpp:487-492
-        self._optimizer = FusedAdam(self._splat_data, lrs, (0.9, 0.999), 1e-15)
+        self._optimizer = make_optimizer(self._splat_data, lrs, p)
         self._scheduler = ExponentialLR(self._optimizer, 0.01 ** (1.0 / p.iterations), 0)
         cap = self._splat_data.capacity
         i64 = lambda n: torch.empty(n, dtype=torch.int64, device=dev)
@@ -197,7 +405,7 @@ class MCMC(IStrategy):
             kept = {n: sd.tensor(n).index_select(0, keep) for n in ("means", "sh0", "shN", "scaling_raw", "rotation_raw", "opacity_raw")}
             sd.size = new_n
             for n, t in kept.items():
-                sd.tensor(n).copy_(t)
+                sd.put(n, t)
         self.grads.size = new_n
         self._grads_valid = False
 
@@ -223,9 +431,14 @@ class MCMC(IStrategy):
              ptr(self._counts), ptr(self._ratios), ptr(self._s_opac), ptr(self._s_scales), st)
         call("lfs_relocation", n, ptr(self._s_opac), ptr(self._s_scales), ptr(self._ratios), ptr(self._binoms), 51,
              ptr(self._new_opac), ptr(self._new_scales), st)
-        p, m, v = sd.struct(), opt.exp_avg.struct(), opt.exp_avg_sq.struct()
+        p = sd.struct()
+        packed = isinstance(opt.exp_avg, PackedMoments)
+        m, v = (None, None) if packed else (C.byref(opt.exp_avg.struct()), C.byref(opt.exp_avg_sq.struct()))
         call("lfs_mcmc_apply", N, sd.K, n, ptr(sampled), ptr(dst), ptr(self._new_opac), ptr(self._new_scales),
-             float(self._params.min_opacity), C.byref(p), C.byref(m), C.byref(v), st)
+             float(self._params.min_opacity), C.byref(p), m, v, st)
+        if packed:
+            for x in (opt.exp_avg, opt.exp_avg_sq):
+                x.zero_rows(slice(N, N + n) if dst is None else sampled[:n])
 
     def relocate_gs(self, sampled_local: torch.Tensor | None = None) -> int:
         """mcmc.cpp:112-190. `sampled_local` (indices into the alive list) may be injected for tests."""
@@ -281,7 +494,7 @@ def _rewrite_rows(buffers, new_rows: dict, new_n: int):
             raise RuntimeError("SplatData capacity exhausted: reserve more rows")
         sd.size = new_n
         for name, t in rows.items():
-            sd.tensor(name).copy_(t.reshape(sd.tensor(name).shape))
+            sd.put(name, t)
 
 
 class DefaultStrategy(IStrategy):
@@ -317,7 +530,7 @@ class DefaultStrategy(IStrategy):
         sd = self._splat_data
         self.densification_info = torch.zeros((2, sd.size), dtype=torch.float32, device=sd.device)
         lrs = [p.means_lr * p.scene_scale, p.shs_lr, p.shs_lr / 20.0, p.scaling_lr, p.rotation_lr, p.opacity_lr]
-        self._optimizer = FusedAdam(sd, lrs, (0.9, 0.999), 1e-15)
+        self._optimizer = make_optimizer(sd, lrs, p)
         self._scheduler = ExponentialLR(self._optimizer, 0.01 ** (1.0 / p.iterations), 0)
 
     def is_refining(self, iter: int) -> bool:
@@ -473,5 +686,5 @@ class DefaultStrategy(IStrategy):
         thr = torch.logit(torch.tensor(2.0 * self._params.prune_opacity)).item()
         self._sync_sizes()
         self._splat_data.tensor("opacity_raw").clamp_(max=thr)
-        self._optimizer.exp_avg.tensor("opacity_raw").zero_()
-        self._optimizer.exp_avg_sq.tensor("opacity_raw").zero_()
+        for moment in (self._optimizer.exp_avg, self._optimizer.exp_avg_sq):
+            moment.put("opacity_raw", torch.zeros_like(moment.tensor("opacity_raw")))

@@ -13,7 +13,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from . import _capi as capi
+from . import _capi as capi, ops
 from ._capi import RenderConfig, UTParams, call, ptr, splats_struct
 
 PARAM_NAMES = ("means", "sh0", "shN", "scaling_raw", "rotation_raw", "opacity_raw")
@@ -72,6 +72,10 @@ class SplatData:
         for n in PARAM_NAMES:
             self.tensor(n).copy_(torch.as_tensor(params[n]).to(self.device).reshape(self.tensor(n).shape))
         return self
+
+    def put(self, name: str, rows: torch.Tensor):
+        """Overwrites the live rows of one group."""
+        self.tensor(name).copy_(rows.reshape(self.tensor(name).shape))
 
     def struct(self) -> capi.Splats:
         return capi.Splats(*(self._full[n].data_ptr() for n in PARAM_NAMES))
@@ -382,6 +386,47 @@ class FastRasterizer:
                     color=rec[:, 6:9], instance_ids=grab(view.instance_ids, n_inst, torch.int32),
                     tile_offsets=grab(view.tile_offsets, tiles + 1, torch.int32),
                     n_contrib=grab(view.n_contrib, self.W * self.H, torch.int32).view(self.H, self.W), n_instances=n_inst)
+
+
+class ShPalette:
+    """Higher-order SH rows that Gaussians share, as the reference's compressed scenes store them (cluster centres and one label per
+    Gaussian, kernels/kmeans.cu): shN[g] = table[labels[g]]. For fine-tuning the palette after densification has ended:
+
+        palette.expand(model); render, loss, backward into grads; palette.backward(grads); AdamW([palette.table], [palette.grad]).step()
+
+    table [rows, K-1, 3] float32, labels [N] int32 or int64; a label that names no row (-1) gives zeros and no gradient. The labels' order is
+    made once here: set_labels for new ones."""
+
+    def __init__(self, table: torch.Tensor, labels: torch.Tensor):
+        if table.dim() != 3 or table.shape[2] != 3 or table.dtype != torch.float32:
+            raise RuntimeError(f"table must be float32 [rows, K-1, 3], got {table.dtype} {list(table.shape)}")
+        ops._check_typed(table, "table", (torch.float32,))
+        self.table = table
+        self.grad = torch.zeros_like(table)
+        self.set_labels(labels)
+
+    def set_labels(self, labels: torch.Tensor):
+        if labels.dim() != 1:
+            raise RuntimeError("labels must be one-dimensional")
+        if labels.device != self.table.device:
+            raise RuntimeError(f"labels must be on {self.table.device}")
+        self.order = ops.embedding_sort(labels, self.table.shape[0])
+        self.labels = labels
+
+    def _rows(self, data: SplatData) -> torch.Tensor:
+        if data.size != self.labels.numel() or data.K - 1 != self.table.shape[1]:
+            raise RuntimeError(f"the palette is for {self.labels.numel()} Gaussians with {self.table.shape[1] + 1} SH bases, got {data.size} with {data.K}")
+        return data.tensor("shN")
+
+    def expand(self, model: SplatData):
+        """Writes every Gaussian's shN row."""
+        ops.embedding_fwd(self.table.flatten(1), self.labels, out=self._rows(model))
+
+    def backward(self, grads: SplatData, accumulate: bool = False) -> torch.Tensor:
+        """The gradient of the table from that of the shN rows (a backward that writes shN), into self.grad."""
+        v = self._rows(grads)
+        ops.embedding_bwd(v.view(v.shape[0], -1), self.order, out=self.grad, accumulate=accumulate)
+        return self.grad
 
 
 class PhotometricLoss:
