@@ -51,6 +51,7 @@ struct AdamWArgs {
     float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, bc2_sqrt_rcp, grad_scale;
     uint32_t offset_m, offset_v;   // the step's part of the rounding thresholds
 };
+constexpr int kCtas8 = 5, kCtas32 = 6;   // CTAs per SM that the registers are shared by
 // under 4 KB and under 32 KB of arguments, which is what a launch takes
 constexpr int kAdamWFew = 32, kAdamWMany = 384;
 
@@ -58,70 +59,90 @@ constexpr uint32_t kGolden = 0x9E3779B9u, kPlastic = 0xC13FA9A9u, kPlastic2 = 0x
 constexpr float kTopM = 448.0f, kTopV = 57344.0f;
 constexpr float kTiny = 0x1p-110f;   // below it a scale would not be a normal number; such a block is held as zeros
 
-struct Block4 { float x[4]; };
+// Two 32-bit operations to an instruction, each rounded as the single one is.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void unpair(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) { f32x2 r; asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
+// A lane's four elements.
+struct Block4 {
+    float x[4];
+    __device__ __forceinline__ f32x2 get(int k) const { return pair(x[2 * k], x[2 * k + 1]); }
+    __device__ __forceinline__ void set(int k, f32x2 v) { unpair(v, x[2 * k], x[2 * k + 1]); }
+};
+__device__ __forceinline__ Block4 times(const Block4& b, float y) {
+    Block4 r;
+    r.set(0, mul2(b.get(0), pair(y, y)));
+    r.set(1, mul2(b.get(1), pair(y, y)));
+    return r;
+}
 
 // ---- 8-bit codes -------------------------------------------------------------------------------
-// `a` in [0, top]: its bits, the threshold added to those that go, shifted. Below the lowest binade the codes are evenly spaced: adding its start gives
-// the number that spacing as last place, and the code is counted from there.
-template <int DROPPED, int LOWEST>
-__device__ __forceinline__ uint32_t round_code(float a, uint32_t threshold) {
-    constexpr float kLeast = LOWEST == -6 ? 0x1p-6f : 0x1p-14f;
-    static_assert(LOWEST == -6 || LOWEST == -14, "");
-    const bool small = a < kLeast;
-    const float t = small ? __fadd_rn(a, kLeast) : a;
-    return ((__float_as_uint(t) + threshold) >> DROPPED) - ((uint32_t)(126 + LOWEST + (small ? 1 : 0)) << (23 - DROPPED));
+// Both codes are float32 with a shorter exponent and fraction. Multiplied by 2^-120 (2^-112) their smallest normal number becomes float32's, and below it both are evenly spaced, so a code is the
+// upper bits of the scaled value, and rounding adds the threshold to the bits that go.
+constexpr float kShiftM = 0x1p-120f, kShiftV = 0x1p-112f;
+constexpr int kDroppedM = 20, kDroppedV = 21;
+
+__device__ __forceinline__ Block4 decode4(uint32_t codes, __nv_fp8_interpretation_t kind, float scale) {
+    const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xFFFFu), kind)));
+    const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), kind)));
+    return times(Block4{{lo.x, lo.y, hi.x, hi.y}}, scale);
 }
-__device__ __forceinline__ uint32_t encode_m(float x, float inverse, uint32_t threshold) {
-    if (!isfinite(x)) return 0x7F;
-    const uint32_t c = round_code<20, -6>(fminf(__fmul_rn(fabsf(x), inverse), kTopM), threshold);
-    return c | ((__float_as_uint(x) >> 24) & 0x80u);
-}
-__device__ __forceinline__ uint32_t encode_v(float x, float inverse, uint32_t threshold) {
-    if (!isfinite(x)) return isinf(x) ? 0x7C : 0x7F;
-    const uint32_t c = round_code<21, -14>(fminf(__fmul_rn(fabsf(x), inverse), kTopV), threshold);
-    return x > 0.0f && inverse > 0.0f ? max(c, 1u) : c;
-}
-__device__ __forceinline__ Block4 decode_m(uint32_t codes, float scale) {
-    const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xFFFFu), __NV_E4M3)));
-    const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E4M3)));
-    return {__fmul_rn(lo.x, scale), __fmul_rn(lo.y, scale), __fmul_rn(hi.x, scale), __fmul_rn(hi.y, scale)};
-}
-__device__ __forceinline__ Block4 decode_v(uint32_t codes, float scale) {
-    const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xFFFFu), __NV_E5M2)));
-    const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E5M2)));
-    return {__fmul_rn(lo.x, scale), __fmul_rn(lo.y, scale), __fmul_rn(hi.x, scale), __fmul_rn(hi.y, scale)};
-}
-// largest finite magnitude of the warp's block; the bits of numbers that are not negative are ordered like the numbers
-__device__ __forceinline__ float block_max(const Block4& b) {
-    uint32_t most = 0;
+__device__ __forceinline__ Block4 decode_m(uint32_t codes, float scale) { return decode4(codes, __NV_E4M3, scale); }
+__device__ __forceinline__ Block4 decode_v(uint32_t codes, float scale) { return decode4(codes, __NV_E5M2, scale); }
+
+__device__ __forceinline__ float max_or_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+// the largest of the warp's numbers, none of them negative; their bits are ordered like the numbers, and NaN above all
+__device__ __forceinline__ float warp_max(float x) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x))); }
+__device__ __forceinline__ float finite_or_zero(float x) { return isfinite(x) ? fabsf(x) : 0.0f; }
+
+// The codes of the warp's block, four a lane, and its scale. `e`: the lane's first element; `offset`: the step's part of the thresholds; `nearest`: half a code's distance instead.
+template <bool SECOND>
+__device__ __forceinline__ uint32_t encode4(const Block4& b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
+    constexpr float kTop = SECOND ? kTopV : kTopM, kTopRcp = 1.0f / kTop, kShift = SECOND ? kShiftV : kShiftM;
+    constexpr int kDropped = SECOND ? kDroppedV : kDroppedM;
+    constexpr uint32_t kStep = SECOND ? kGolden : kPlastic2;
+    float most = warp_max(max_or_nan(max_or_nan(fabsf(b.x[0]), fabsf(b.x[1])), max_or_nan(fabsf(b.x[2]), fabsf(b.x[3]))));
+    const bool finite = isfinite(most);
+    if (!finite) most = warp_max(fmaxf(fmaxf(finite_or_zero(b.x[0]), finite_or_zero(b.x[1])), fmaxf(finite_or_zero(b.x[2]), finite_or_zero(b.x[3]))));
+    const bool held = most >= kTiny;
+    const float inverse = held ? __fdiv_rn(kTop, most) : 0.0f;
+    *scale = held ? __fmul_rn(most, kTopRcp) : 0.0f;
+    Block4 y = times(b, inverse);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) most = max(most, isfinite(b.x[k]) ? __float_as_uint(fabsf(b.x[k])) : 0u);
-    return __uint_as_float(__reduce_max_sync(0xffffffffu, most));
-}
-struct Scaling { float inverse, scale; };
-__device__ __forceinline__ Scaling block_scaling(float most, float top, float top_rcp) {
-    if (most < kTiny) return {0.0f, 0.0f};
-    return {__fdiv_rn(top, most), __fmul_rn(most, top_rcp)};
-}
-// codes of the warp's block, four a lane. `offset`: the step's part of the thresholds; `nearest`: half a code's distance instead.
-__device__ __forceinline__ uint32_t encode_block_m(const Block4& b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
-    const Scaling s = block_scaling(block_max(b), kTopM, 1.0f / kTopM);
-    *scale = s.scale;
-    uint32_t codes = 0;
+    for (int k = 0; k < 4; ++k) y.x[k] = fminf(fabsf(y.x[k]), kTop);
+    y = times(y, kShift);
+    uint32_t h = e * kStep + offset, codes = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) codes |= encode_m(b.x[k], s.inverse, nearest ? 1u << 19 : ((e + k) * kPlastic2 + offset) >> 12) << (8 * k);
-    return codes;
-}
-__device__ __forceinline__ uint32_t encode_block_v(const Block4& b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
-    const Scaling s = block_scaling(block_max(b), kTopV, 1.0f / kTopV);
-    *scale = s.scale;
-    uint32_t codes = 0;
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t threshold = nearest ? 1u << (kDropped - 1) : h >> (32 - kDropped);
+        codes |= ((__float_as_uint(y.x[k]) + threshold) >> kDropped) << (8 * k);
+        h += kStep;
+    }
+    if (SECOND) {   // what is not zero is not held as zero
+        if (held && ((codes - 0x01010101u) & ~codes & 0x80808080u)) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) codes |= encode_v(b.x[k], s.inverse, nearest ? 1u << 20 : ((e + k) * kGolden + offset) >> 11) << (8 * k);
+            for (int k = 0; k < 4; ++k)
+                if (b.x[k] > 0.0f && !((codes >> (8 * k)) & 0xFF)) codes |= 1u << (8 * k);
+        }
+    } else {
+        const uint32_t lo = __byte_perm(__float_as_uint(b.x[0]), __float_as_uint(b.x[1]), 0x0073), hi = __byte_perm(__float_as_uint(b.x[2]), __float_as_uint(b.x[3]), 0x7300);
+        codes |= __byte_perm(lo, hi, 0x7610) & 0x80808080u;
+    }
+    if (!finite) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t is = isfinite(b.x[k]) ? (codes >> (8 * k)) & 0xFF : SECOND && isinf(b.x[k]) ? 0x7Cu : 0x7Fu;
+            codes = (codes & ~(0xFFu << (8 * k))) | is << (8 * k);
+        }
+    }
     return codes;
 }
 
-// ---- a lane's four elements ----------------------------------------------------------------------
+// ---- memory ------------------------------------------------------------------------------------------
 __device__ __forceinline__ Block4 load4(const float* src, int64_t e, int64_t n, bool whole) {
     if (whole) {
         const float4 a = *reinterpret_cast<const float4*>(src + e);
@@ -161,66 +182,115 @@ __device__ __forceinline__ void store4(uint8_t* dst, int64_t e, int64_t n, bool 
 __device__ __forceinline__ float half_bits(uint32_t bits, int dtype) {
     return dtype == LFS_BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
 }
-__device__ __forceinline__ Block4 load_grad(const void* src, int dtype, int64_t e, int64_t n, bool whole) {
-    if (dtype == LFS_F32) return load4(static_cast<const float*>(src), e, n, whole);
+__device__ __forceinline__ float fast_root(float x) { float r; asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float fast_reciprocal(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
+// A lane's part of a block as it lies in memory.
+template <int BITS>
+struct Raw {
+    Block4 p;
+    uint4 g;                         // four floats, or four 16-bit numbers in x and y
+    Block4 m32, v32;                 // BITS 32
+    uint32_t m8, v8;                 // BITS 8
+    float ms, vs;
+};
+__device__ __forceinline__ Block4 gradients(const uint4& g, int dtype) {
+    if (dtype == LFS_F32) return {__uint_as_float(g.x), __uint_as_float(g.y), __uint_as_float(g.z), __uint_as_float(g.w)};
+    return {half_bits(g.x & 0xFFFFu, dtype), half_bits(g.x >> 16, dtype), half_bits(g.y & 0xFFFFu, dtype), half_bits(g.y >> 16, dtype)};
+}
+__device__ __forceinline__ uint4 load_grad(const void* src, int dtype, int64_t e, int64_t n, bool whole) {
+    if (dtype == LFS_F32) {
+        const Block4 g = load4(static_cast<const float*>(src), e, n, whole);
+        return make_uint4(__float_as_uint(g.x[0]), __float_as_uint(g.x[1]), __float_as_uint(g.x[2]), __float_as_uint(g.x[3]));
+    }
     const uint16_t* h = static_cast<const uint16_t*>(src);
     if (whole) {
         const uint2 w = *reinterpret_cast<const uint2*>(h + e);
-        return {half_bits(w.x & 0xFFFFu, dtype), half_bits(w.x >> 16, dtype), half_bits(w.y & 0xFFFFu, dtype), half_bits(w.y >> 16, dtype)};
+        return make_uint4(w.x, w.y, 0, 0);
     }
-    Block4 b;
+    uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) b.x[k] = e + k < n ? half_bits(h[e + k], dtype) : 0.0f;
-    return b;
+    for (int k = 0; k < 4; ++k) w[k] = e + k < n ? h[e + k] : 0;
+    return make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, 0, 0);
+}
+template <int BITS>
+__device__ __forceinline__ void load_raw(Raw<BITS>& r, const AdamWTensor& T, int64_t start, int64_t e, bool whole) {
+    r.p = load4(T.p, e, T.n, whole);
+    r.g = load_grad(T.g, T.grad_dtype, e, T.n, whole);
+    if constexpr (BITS == 8) {
+        r.m8 = load4(static_cast<const uint8_t*>(T.m), e, T.n, whole);
+        r.v8 = load4(static_cast<const uint8_t*>(T.v), e, T.n, whole);
+        r.ms = T.ms[start / kAdamWBlock];
+        r.vs = T.vs[start / kAdamWBlock];
+    } else {
+        r.m32 = load4(static_cast<const float*>(T.m), e, T.n, whole);
+        r.v32 = load4(static_cast<const float*>(T.v), e, T.n, whole);
+    }
 }
 
-template <int CAP>
-__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
+// One warp per block, the next one's loads under way while a block is computed.
+template <int CAP, int BITS>
+__global__ void __launch_bounds__(256, BITS == 8 ? kCtas8 : kCtas32) adamw_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
     const int lane = threadIdx.x & 31;
     const int warps = (int)(gridDim.x * (blockDim.x >> 5));
     const int total = A.first[A.n];
-    int k = 0;
-    for (int q = (int)(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)); q < total; q += warps) {
-        while (q >= A.first[k + 1]) ++k;
-        const AdamWTensor& T = A.t[k];
-        const int64_t start = (int64_t)(q - A.first[k]) * kAdamWBlock, e = start + lane * 4;
-        const bool whole = T.aligned && start + kAdamWBlock <= T.n;
-        Block4 p = load4(T.p, e, T.n, whole);
-        const Block4 g = load_grad(T.g, T.grad_dtype, e, T.n, whole);
-        Block4 m, v;
-        if (T.ms) {
-            const int64_t b = start / kAdamWBlock;
-            m = decode_m(load4(static_cast<const uint8_t*>(T.m), e, T.n, whole), T.ms[b]);
-            v = decode_v(load4(static_cast<const uint8_t*>(T.v), e, T.n, whole), T.vs[b]);
+    int q = (int)(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)), next = 0;
+    if (q >= total) return;
+    while (q >= A.first[next + 1]) ++next;
+    Raw<BITS> r;
+    int64_t start = (int64_t)(q - A.first[next]) * kAdamWBlock;
+    load_raw<BITS>(r, A.t[next], start, start + lane * 4, A.t[next].aligned && start + kAdamWBlock <= A.t[next].n);
+    for (;;) {
+        const AdamWTensor& T = A.t[next];
+        const int64_t at = start, e = at + lane * 4;
+        const bool whole = T.aligned && at + kAdamWBlock <= T.n;
+        Block4 p = r.p, m, v;
+        const Block4 g = gradients(r.g, T.grad_dtype);
+        if constexpr (BITS == 8) {
+            m = decode_m(r.m8, r.ms);
+            v = decode_v(r.v8, r.vs);
         } else {
-            m = load4(static_cast<const float*>(T.m), e, T.n, whole);
-            v = load4(static_cast<const float*>(T.v), e, T.n, whole);
+            m = r.m32;
+            v = r.v32;
+        }
+        q += warps;
+        const bool more = q < total;
+        if (more) {
+            while (q >= A.first[next + 1]) ++next;
+            start = (int64_t)(q - A.first[next]) * kAdamWBlock;
+            load_raw<BITS>(r, A.t[next], start, start + lane * 4, A.t[next].aligned && start + kAdamWBlock <= A.t[next].n);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float gs = __fmul_rn(g.x[i], A.grad_scale);
-            m.x[i] = __fadd_rn(__fmul_rn(m.x[i], A.beta1), __fmul_rn(gs, A.one_minus_beta1));
-            v.x[i] = __fadd_rn(__fmul_rn(v.x[i], A.beta2), __fmul_rn(__fmul_rn(gs, A.one_minus_beta2), gs));
-            const float denom = __fadd_rn(__fmul_rn(__fsqrt_rn(v.x[i]), A.bc2_sqrt_rcp), A.eps);
-            p.x[i] = __fsub_rn(__fmul_rn(p.x[i], T.decay), __fdiv_rn(__fmul_rn(m.x[i], T.step_size), denom));
+        for (int i = 0; i < 2; ++i) {
+            const f32x2 gs = mul2(g.get(i), pair(A.grad_scale, A.grad_scale));
+            const f32x2 m1 = add2(mul2(m.get(i), pair(A.beta1, A.beta1)), mul2(gs, pair(A.one_minus_beta1, A.one_minus_beta1)));
+            const f32x2 v1 = add2(mul2(v.get(i), pair(A.beta2, A.beta2)), mul2(mul2(gs, pair(A.one_minus_beta2, A.one_minus_beta2)), gs));
+            m.set(i, m1);
+            v.set(i, v1);
+            // The moments are rounded step by step, since their codes depend on it; the step itself takes the fast root and reciprocal, which are off by 2^-23 of it
+            // (exact ones: two thirds more instructions). A denominator is zero or normal: the root of the smallest number is 2^-74.5.
+            float a, b;
+            unpair(add2(mul2(pair(fast_root(v.x[2 * i]), fast_root(v.x[2 * i + 1])), pair(A.bc2_sqrt_rcp, A.bc2_sqrt_rcp)), pair(A.eps, A.eps)), a, b);
+            const f32x2 step = mul2(mul2(m1, pair(T.step_size, T.step_size)), pair(fast_reciprocal(a), fast_reciprocal(b)));
+            p.set(i, sub2(mul2(p.get(i), pair(T.decay, T.decay)), step));
         }
         store4(T.p, e, T.n, whole, p);
-        if (T.ms) {
-            const int64_t b = start / kAdamWBlock;
+        if constexpr (BITS == 8) {
             float ms, vs;
-            if (!whole)   // what lies behind the tensor's end has no part in the scale (0/0 above where eps is zero)
+            if (!whole)   // what lies behind the tensor's end has no part in the scale
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (e + i >= T.n) m.x[i] = v.x[i] = 0.0f;
-            const uint32_t mc = encode_block_m(m, (uint32_t)e, A.offset_m, false, &ms);
-            const uint32_t vc = encode_block_v(v, (uint32_t)e, A.offset_v, false, &vs);
+            const uint32_t mc = encode4<false>(m, (uint32_t)e, A.offset_m, false, &ms);
+            const uint32_t vc = encode4<true>(v, (uint32_t)e, A.offset_v, false, &vs);
             store4(static_cast<uint8_t*>(T.m), e, T.n, whole, mc);
             store4(static_cast<uint8_t*>(T.v), e, T.n, whole, vc);
-            if (lane == 0) { T.ms[b] = ms; T.vs[b] = vs; }
+            if (lane == 0) { T.ms[at / kAdamWBlock] = ms; T.vs[at / kAdamWBlock] = vs; }
         } else {
             store4(static_cast<float*>(T.m), e, T.n, whole, m);
             store4(static_cast<float*>(T.v), e, T.n, whole, v);
         }
+        if (!more) return;
     }
 }
 
@@ -232,7 +302,7 @@ __global__ void __launch_bounds__(256) adamw_encode_kernel(int64_t n, int64_t bl
         const bool whole = aligned && (b + 1) * kAdamWBlock <= n;
         const Block4 x = load4(values, e, n, whole);
         float scale;
-        const uint32_t c = second ? encode_block_v(x, 0, 0, true, &scale) : encode_block_m(x, 0, 0, true, &scale);
+        const uint32_t c = second ? encode4<true>(x, 0, 0, true, &scale) : encode4<false>(x, 0, 0, true, &scale);
         store4(codes, e, n, whole, c);
         if (lane == 0) scales[b] = scale;
     }
@@ -249,56 +319,63 @@ __global__ void __launch_bounds__(256) adamw_decode_kernel(int64_t n, int64_t bl
     }
 }
 
-template <int CAP>
-int launch_adamw(int count, const lfs_adamw_tensor* tensors, double beta1, double beta2, double eps, int64_t step_count, float grad_scale, cudaStream_t st) {
+// One launch over the tensors of one kind of moments (every tensor of a list, or those that are left when the other kind has been taken out).
+template <int CAP, int BITS>
+int launch_adamw(int count, const lfs_adamw_tensor* const* tensors, double beta1, double beta2, double eps, int64_t step_count, float grad_scale, cudaStream_t st) {
     static_assert(sizeof(AdamWArgs<CAP>) <= 32764, "kernel arguments");
     // the same host arithmetic as lfs_adam_step_segments
     const double bc1 = 1.0 / (1.0 - std::pow(beta1, (double)step_count));
     const double bc2 = 1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step_count));
     AdamWArgs<CAP> A;
     int64_t blocks = 0;
-    A.n = 0;
+    A.n = count;
     A.first[0] = 0;
     for (int k = 0; k < count; ++k) {
-        const lfs_adamw_tensor& t = tensors[k];
-        if (t.n == 0) continue;
-        AdamWTensor& o = A.t[A.n];
+        const lfs_adamw_tensor& t = *tensors[k];
+        AdamWTensor& o = A.t[k];
         o.p = t.param; o.g = t.grad; o.m = t.exp_avg; o.v = t.exp_avg_sq; o.ms = t.exp_avg_scale; o.vs = t.exp_avg_sq_scale;
         o.n = t.n;
         o.step_size = (float)((double)t.lr * bc1);
         o.decay = (float)(1.0 - (double)t.lr * (double)t.weight_decay);
         o.grad_dtype = t.grad_dtype;
-        const uintptr_t moment = t.exp_avg_scale ? 4 : 16;
+        const uintptr_t moment = BITS == 8 ? 4 : 16;
         o.aligned = aligned_by(t.param, 16) && aligned_by(t.grad, 4 * dtype_bytes(t.grad_dtype)) && aligned_by(t.exp_avg, moment) && aligned_by(t.exp_avg_sq, moment);
         blocks += (t.n + kAdamWBlock - 1) / kAdamWBlock;
         if (blocks >= (int64_t)1 << 30) {
             set_error("lfs_adamw_step_tensors: more than 2^37 elements in one launch");
             return LFS_EINVAL;
         }
-        A.first[++A.n] = (int32_t)blocks;
+        A.first[k + 1] = (int32_t)blocks;
     }
-    if (blocks == 0) return LFS_OK;
     A.beta1 = (float)beta1; A.beta2 = (float)beta2;
     A.one_minus_beta1 = (float)(1.0 - beta1); A.one_minus_beta2 = (float)(1.0 - beta2);
     A.eps = (float)eps; A.bc2_sqrt_rcp = (float)bc2; A.grad_scale = grad_scale;
     A.offset_m = (uint32_t)step_count * kGolden;
     A.offset_v = (uint32_t)step_count * kPlastic;
     LFS_TIMED("adamw", st);
-    adamw_kernel<CAP><<<grid_for(blocks, 8, 8), 256, 0, st>>>(A);
+    adamw_kernel<CAP, BITS><<<grid_for(blocks, 8, BITS == 8 ? kCtas8 : kCtas32), 256, 0, st>>>(A);
     return check_launch("adamw");
+}
+template <int BITS>
+int launch_adamw_kind(int n_tensors, const lfs_adamw_tensor* tensors, double beta1, double beta2, double eps, int64_t step_count, float grad_scale, cudaStream_t st) {
+    const lfs_adamw_tensor* some[kAdamWMany];
+    for (int k = 0; k < n_tensors;) {
+        int count = 0;
+        for (; k < n_tensors && count < kAdamWMany; ++k)
+            if (tensors[k].n > 0 && (tensors[k].exp_avg_scale != nullptr) == (BITS == 8)) some[count++] = tensors + k;
+        if (count == 0) continue;
+        const int rc = (count <= kAdamWFew ? launch_adamw<kAdamWFew, BITS> : launch_adamw<kAdamWMany, BITS>)(count, some, beta1, beta2, eps, step_count, grad_scale, st);
+        if (rc != LFS_OK) return rc;
+    }
+    return LFS_OK;
 }
 
 }  // namespace
 
 int launch_adamw_tensors(int n_tensors, const lfs_adamw_tensor* tensors, double beta1, double beta2, double eps, int64_t step_count, float grad_scale,
                          cudaStream_t st) {
-    for (int k = 0; k < n_tensors;) {
-        const int count = n_tensors - k < kAdamWMany ? n_tensors - k : kAdamWMany;
-        const int rc = (count <= kAdamWFew ? launch_adamw<kAdamWFew> : launch_adamw<kAdamWMany>)(count, tensors + k, beta1, beta2, eps, step_count, grad_scale, st);
-        if (rc != LFS_OK) return rc;
-        k += count;
-    }
-    return LFS_OK;
+    const int rc = launch_adamw_kind<32>(n_tensors, tensors, beta1, beta2, eps, step_count, grad_scale, st);
+    return rc != LFS_OK ? rc : launch_adamw_kind<8>(n_tensors, tensors, beta1, beta2, eps, step_count, grad_scale, st);
 }
 
 int launch_adamw_encode(int64_t n, const float* values, int second_moment, uint8_t* codes, float* scales, cudaStream_t st) {
