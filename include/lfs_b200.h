@@ -416,7 +416,7 @@ typedef struct lfs_adam_segment {
 int lfs_adam_step_segments(int n_segments, const lfs_adam_segment* segments /* host */, double beta1, double beta2,
                            double eps, int64_t step_count, float grad_scale, int ctas_per_sm, void* stream);
 
-/* AdamW (Adam with decoupled weight decay) over any number of contiguous tensors, one launch per 384 of them (no counterpart
+/* AdamW (Adam with decoupled weight decay) over any number of contiguous tensors, one launch per 424 of them (no counterpart
  * in the reference, whose optimizer has no weight decay and keeps 32-bit moments): what is trained next to the Gaussians (per-image
  * codes, exposure matrices, bilateral grids, palettes, small networks) and scenes whose moments should take a quarter of
  * the memory. With g = grad_scale * grad, t = step_count >= 1:

@@ -17,6 +17,8 @@
 // Explicit roundings (no contracted products), so that a code does not depend on how the compiler forms an expression.
 #include "optim.cuh"
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include <cuda_bf16.h>
@@ -35,25 +37,30 @@ struct AdamWTensor {
     const void* g;
     void *m, *v;          // float, or e4m3 and e5m2 codes
     float *ms, *vs;       // scales of the blocks; null with 32-bit moments
-    int64_t n;
+    uint32_t n;
+    uint32_t before;      // elements in front of these where a tensor is longer than kPiece, modulo 2^32
     float step_size;      // lr / (1 - beta1^t)
     float decay;          // 1 - lr * weight decay
     int32_t grad_dtype;
     int32_t aligned;      // whole vectors can be read and written
 };
+constexpr int64_t kPiece = (int64_t)1 << 30;
 
 // A kernel takes its tensors as an argument: nothing is copied to the device or kept there, and a captured launch has its own copy.
 template <int CAP>
 struct AdamWArgs {
     AdamWTensor t[CAP];
-    int32_t first[CAP + 1];   // blocks in front of tensor k
+    int32_t first[CAP + 1];   // tiles in front of tensor k
     int32_t n;
     float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, bc2_sqrt_rcp, grad_scale;
     uint32_t offset_m, offset_v;   // the step's part of the rounding thresholds
 };
-constexpr int kCtas8 = 5, kCtas32 = 6;   // CTAs per SM that the registers are shared by
 // under 4 KB and under 32 KB of arguments, which is what a launch takes
-constexpr int kAdamWFew = 32, kAdamWMany = 384;
+constexpr int kAdamWFew = 32, kAdamWMany = 424;
+
+// A CTA takes a tile of kTile elements at a time, kBlocks blocks to a warp, with the next ones being copied to shared memory.
+constexpr int kWarps = 8, kThreads = kWarps * 32, kBlocks = 2, kRow = kWarps * kAdamWBlock, kTile = kBlocks * kRow;
+constexpr int kStages = 2, kCtas8 = 4, kCtas32 = 3;
 
 constexpr uint32_t kGolden = 0x9E3779B9u, kPlastic = 0xC13FA9A9u, kPlastic2 = 0x91E10DA5u;
 constexpr float kTopM = 448.0f, kTopV = 57344.0f;
@@ -95,35 +102,38 @@ __device__ __forceinline__ Block4 decode_m(uint32_t codes, float scale) { return
 __device__ __forceinline__ Block4 decode_v(uint32_t codes, float scale) { return decode4(codes, __NV_E5M2, scale); }
 
 __device__ __forceinline__ float max_or_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float max4(const Block4& b) {
+    return max_or_nan(max_or_nan(fabsf(b.x[0]), fabsf(b.x[1])), max_or_nan(fabsf(b.x[2]), fabsf(b.x[3])));
+}
 // the largest of the warp's numbers, none of them negative; their bits are ordered like the numbers, and NaN above all
 __device__ __forceinline__ float warp_max(float x) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x))); }
-__device__ __forceinline__ float finite_or_zero(float x) { return isfinite(x) ? fabsf(x) : 0.0f; }
 
-// The codes of the warp's block, four a lane, and its scale. `e`: the lane's first element; `offset`: the step's part of the thresholds; `nearest`: half a code's distance instead.
+struct Scaling { float inverse, scale; };
 template <bool SECOND>
-__device__ __forceinline__ uint32_t encode4(const Block4& b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
-    constexpr float kTop = SECOND ? kTopV : kTopM, kTopRcp = 1.0f / kTop, kShift = SECOND ? kShiftV : kShiftM;
+__device__ __forceinline__ Scaling scaling(float most) {
+    constexpr float kTop = SECOND ? kTopV : kTopM, kTopRcp = 1.0f / kTop;
+    const bool held = most >= kTiny;
+    return {held ? __fdiv_rn(kTop, most) : 0.0f, held ? __fmul_rn(most, kTopRcp) : 0.0f};
+}
+// A lane's four codes. `e`: its first element; `offset`: the step's part of the thresholds; `nearest`: half a code's distance instead. What is not finite is left to the caller.
+template <bool SECOND>
+__device__ __forceinline__ uint32_t encode4(const Block4& b, float inverse, uint32_t e, uint32_t offset, bool nearest) {
+    constexpr float kTop = SECOND ? kTopV : kTopM, kShift = SECOND ? kShiftV : kShiftM;
     constexpr int kDropped = SECOND ? kDroppedV : kDroppedM;
     constexpr uint32_t kStep = SECOND ? kGolden : kPlastic2;
-    float most = warp_max(max_or_nan(max_or_nan(fabsf(b.x[0]), fabsf(b.x[1])), max_or_nan(fabsf(b.x[2]), fabsf(b.x[3]))));
-    const bool finite = isfinite(most);
-    if (!finite) most = warp_max(fmaxf(fmaxf(finite_or_zero(b.x[0]), finite_or_zero(b.x[1])), fmaxf(finite_or_zero(b.x[2]), finite_or_zero(b.x[3]))));
-    const bool held = most >= kTiny;
-    const float inverse = held ? __fdiv_rn(kTop, most) : 0.0f;
-    *scale = held ? __fmul_rn(most, kTopRcp) : 0.0f;
     Block4 y = times(b, inverse);
 #pragma unroll
     for (int k = 0; k < 4; ++k) y.x[k] = fminf(fabsf(y.x[k]), kTop);
     y = times(y, kShift);
-    uint32_t h = e * kStep + offset, codes = 0;
+    uint32_t h = e * kStep + offset, c[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const uint32_t threshold = nearest ? 1u << (kDropped - 1) : h >> (32 - kDropped);
-        codes |= ((__float_as_uint(y.x[k]) + threshold) >> kDropped) << (8 * k);
+        c[k] = (__float_as_uint(y.x[k]) + (nearest ? 1u << (kDropped - 1) : h >> (32 - kDropped))) >> kDropped;
         h += kStep;
     }
+    uint32_t codes = (c[0] | c[1] << 8) | (c[2] | c[3] << 8) << 16;
     if (SECOND) {   // what is not zero is not held as zero
-        if (held && ((codes - 0x01010101u) & ~codes & 0x80808080u)) {
+        if (((codes - 0x01010101u) & ~codes & 0x80808080u) && inverse > 0.0f) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 if (b.x[k] > 0.0f && !((codes >> (8 * k)) & 0xFF)) codes |= 1u << (8 * k);
@@ -132,14 +142,29 @@ __device__ __forceinline__ uint32_t encode4(const Block4& b, uint32_t e, uint32_
         const uint32_t lo = __byte_perm(__float_as_uint(b.x[0]), __float_as_uint(b.x[1]), 0x0073), hi = __byte_perm(__float_as_uint(b.x[2]), __float_as_uint(b.x[3]), 0x7300);
         codes |= __byte_perm(lo, hi, 0x7610) & 0x80808080u;
     }
-    if (!finite) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t is = isfinite(b.x[k]) ? (codes >> (8 * k)) & 0xFF : SECOND && isinf(b.x[k]) ? 0x7Cu : 0x7Fu;
-            codes = (codes & ~(0xFFu << (8 * k))) | is << (8 * k);
-        }
-    }
     return codes;
+}
+// A block with numbers that are not finite: the others' scale is theirs alone.
+template <bool SECOND>
+__device__ __noinline__ uint32_t encode4_not_finite(Block4 b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
+    Block4 f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f.x[k] = isfinite(b.x[k]) ? b.x[k] : 0.0f;
+    const Scaling s = scaling<SECOND>(warp_max(max4(f)));
+    *scale = s.scale;
+    uint32_t codes = encode4<SECOND>(f, s.inverse, e, offset, nearest);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (!isfinite(b.x[k])) codes = (codes & ~(0xFFu << (8 * k))) | (SECOND && isinf(b.x[k]) ? 0x7Cu : 0x7Fu) << (8 * k);
+    return codes;
+}
+template <bool SECOND>
+__device__ __forceinline__ uint32_t encode_block(const Block4& b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
+    const float most = warp_max(max4(b));
+    if (!isfinite(most)) return encode4_not_finite<SECOND>(b, e, offset, nearest, scale);
+    const Scaling s = scaling<SECOND>(most);
+    *scale = s.scale;
+    return encode4<SECOND>(b, s.inverse, e, offset, nearest);
 }
 
 // ---- memory ------------------------------------------------------------------------------------------
@@ -185,112 +210,208 @@ __device__ __forceinline__ float half_bits(uint32_t bits, int dtype) {
 __device__ __forceinline__ float fast_root(float x) { float r; asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float fast_reciprocal(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-// A lane's part of a block as it lies in memory.
-template <int BITS>
-struct Raw {
-    Block4 p;
-    uint4 g;                         // four floats, or four 16-bit numbers in x and y
-    Block4 m32, v32;                 // BITS 32
-    uint32_t m8, v8;                 // BITS 8
-    float ms, vs;
+struct Step {
+    float grad_scale, beta1, beta2, one_minus_beta1, one_minus_beta2, bc2_sqrt_rcp, eps, step_size, decay;
 };
-__device__ __forceinline__ Block4 gradients(const uint4& g, int dtype) {
-    if (dtype == LFS_F32) return {__uint_as_float(g.x), __uint_as_float(g.y), __uint_as_float(g.z), __uint_as_float(g.w)};
-    return {half_bits(g.x & 0xFFFFu, dtype), half_bits(g.x >> 16, dtype), half_bits(g.y & 0xFFFFu, dtype), half_bits(g.y >> 16, dtype)};
-}
-__device__ __forceinline__ uint4 load_grad(const void* src, int dtype, int64_t e, int64_t n, bool whole) {
-    if (dtype == LFS_F32) {
-        const Block4 g = load4(static_cast<const float*>(src), e, n, whole);
-        return make_uint4(__float_as_uint(g.x[0]), __float_as_uint(g.x[1]), __float_as_uint(g.x[2]), __float_as_uint(g.x[3]));
-    }
-    const uint16_t* h = static_cast<const uint16_t*>(src);
-    if (whole) {
-        const uint2 w = *reinterpret_cast<const uint2*>(h + e);
-        return make_uint4(w.x, w.y, 0, 0);
-    }
-    uint32_t w[4];
+__device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Block4& g, const Step& S) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = e + k < n ? h[e + k] : 0;
-    return make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, 0, 0);
-}
-template <int BITS>
-__device__ __forceinline__ void load_raw(Raw<BITS>& r, const AdamWTensor& T, int64_t start, int64_t e, bool whole) {
-    r.p = load4(T.p, e, T.n, whole);
-    r.g = load_grad(T.g, T.grad_dtype, e, T.n, whole);
-    if constexpr (BITS == 8) {
-        r.m8 = load4(static_cast<const uint8_t*>(T.m), e, T.n, whole);
-        r.v8 = load4(static_cast<const uint8_t*>(T.v), e, T.n, whole);
-        r.ms = T.ms[start / kAdamWBlock];
-        r.vs = T.vs[start / kAdamWBlock];
-    } else {
-        r.m32 = load4(static_cast<const float*>(T.m), e, T.n, whole);
-        r.v32 = load4(static_cast<const float*>(T.v), e, T.n, whole);
+    for (int i = 0; i < 2; ++i) {
+        const f32x2 gs = mul2(g.get(i), pair(S.grad_scale, S.grad_scale));
+        const f32x2 m1 = add2(mul2(m.get(i), pair(S.beta1, S.beta1)), mul2(gs, pair(S.one_minus_beta1, S.one_minus_beta1)));
+        const f32x2 v1 = add2(mul2(v.get(i), pair(S.beta2, S.beta2)), mul2(mul2(gs, pair(S.one_minus_beta2, S.one_minus_beta2)), gs));
+        m.set(i, m1);
+        v.set(i, v1);
+        // The moments are rounded step by step, since their codes depend on it; the step itself takes the fast root and reciprocal, which are off by 2^-23 of it
+        // (exact ones: two thirds more instructions). A denominator is zero or normal: the root of the smallest number is 2^-74.5.
+        float a, b;
+        unpair(add2(mul2(pair(fast_root(v.x[2 * i]), fast_root(v.x[2 * i + 1])), pair(S.bc2_sqrt_rcp, S.bc2_sqrt_rcp)), pair(S.eps, S.eps)), a, b);
+        const f32x2 step = mul2(mul2(m1, pair(S.step_size, S.step_size)), pair(fast_reciprocal(a), fast_reciprocal(b)));
+        p.set(i, sub2(mul2(p.get(i), pair(S.decay, S.decay)), step));
     }
 }
 
-// One warp per block, the next one's loads under way while a block is computed.
-template <int CAP, int BITS>
-__global__ void __launch_bounds__(256, BITS == 8 ? kCtas8 : kCtas32) adamw_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
-    const int lane = threadIdx.x & 31;
-    const int warps = (int)(gridDim.x * (blockDim.x >> 5));
+// A warp's block of a tile that is not whole, or of a tensor that cannot be read in vectors.
+template <int BITS>
+__device__ __noinline__ void single_block(const AdamWTensor& T, uint32_t start, int lane, const Step& S, uint32_t offset_m, uint32_t offset_v) {
+    const int64_t e = (int64_t)start + lane * 4, n = T.n;
+    const bool whole = T.aligned && start + kAdamWBlock <= T.n;
+    Block4 p = load4(T.p, e, n, whole), g, m, v;
+    if (T.grad_dtype == LFS_F32) g = load4(static_cast<const float*>(T.g), e, n, whole);
+    else
+#pragma unroll
+        for (int k = 0; k < 4; ++k) g.x[k] = e + k < n ? half_bits(static_cast<const uint16_t*>(T.g)[e + k], T.grad_dtype) : 0.0f;
+    if constexpr (BITS == 8) {
+        m = decode_m(load4(static_cast<const uint8_t*>(T.m), e, n, whole), T.ms[start / kAdamWBlock]);
+        v = decode_v(load4(static_cast<const uint8_t*>(T.v), e, n, whole), T.vs[start / kAdamWBlock]);
+    } else {
+        m = load4(static_cast<const float*>(T.m), e, n, whole);
+        v = load4(static_cast<const float*>(T.v), e, n, whole);
+    }
+    update(p, m, v, g, S);
+    store4(T.p, e, n, whole, p);
+    if constexpr (BITS == 8) {
+        // what lies behind the tensor's end has no part in the scale
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (e + k >= n) m.x[k] = v.x[k] = 0.0f;
+        float ms, vs;
+        const uint32_t i = T.before + (uint32_t)e;
+        store4(static_cast<uint8_t*>(T.m), e, n, whole, encode_block<false>(m, i, offset_m, false, &ms));
+        store4(static_cast<uint8_t*>(T.v), e, n, whole, encode_block<true>(v, i, offset_v, false, &vs));
+        if (lane == 0) {
+            T.ms[start / kAdamWBlock] = ms;
+            T.vs[start / kAdamWBlock] = vs;
+        }
+    } else {
+        store4(static_cast<float*>(T.m), e, n, whole, m);
+        store4(static_cast<float*>(T.v), e, n, whole, v);
+    }
+}
+
+// the tensor of tile q, which is not in front of tensor k's
+template <int CAP>
+__device__ __forceinline__ int tensor_of(const AdamWArgs<CAP>& A, int q, int k) {
+    if (q < A.first[k + 1]) return k;
+    int lo = k + 1, hi = A.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (q < A.first[mid + 1]) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+// A tile as it lies in memory; 16-bit gradients fill the first half of g.
+struct Stage {
+    float p[kTile], g[kTile];
+    uint8_t m[kTile], v[kTile];
+    float ms[kTile / kAdamWBlock], vs[kTile / kAdamWBlock];
+};
+static_assert(kThreads * 4 == kRow && kThreads * 16 == 2 * kTile, "one copy of 16 bytes a thread for both codes, and for 16-bit gradients");
+
+// Moments in 8 bits. Issue slots and memory are both near their limits, so the copies are wide and asynchronous: loads straight into registers wait for one another at every block, and cost
+// more instructions for their addresses.
+template <int CAP>
+__global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
+    extern __shared__ __align__(128) char stages_s[];
+    Stage* const stages = reinterpret_cast<Stage*>(stages_s);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x;
     const int total = A.first[A.n];
-    int q = (int)(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)), next = 0;
-    if (q >= total) return;
-    while (q >= A.first[next + 1]) ++next;
-    Raw<BITS> r;
-    int64_t start = (int64_t)(q - A.first[next]) * kAdamWBlock;
-    load_raw<BITS>(r, A.t[next], start, start + lane * 4, A.t[next].aligned && start + kAdamWBlock <= A.t[next].n);
-    for (;;) {
-        const AdamWTensor& T = A.t[next];
-        const int64_t at = start, e = at + lane * 4;
-        const bool whole = T.aligned && at + kAdamWBlock <= T.n;
-        Block4 p = r.p, m, v;
-        const Block4 g = gradients(r.g, T.grad_dtype);
-        if constexpr (BITS == 8) {
-            m = decode_m(r.m8, r.ms);
-            v = decode_v(r.v8, r.vs);
-        } else {
-            m = r.m32;
-            v = r.v32;
-        }
-        q += warps;
-        const bool more = q < total;
-        if (more) {
-            while (q >= A.first[next + 1]) ++next;
-            start = (int64_t)(q - A.first[next]) * kAdamWBlock;
-            load_raw<BITS>(r, A.t[next], start, start + lane * 4, A.t[next].aligned && start + kAdamWBlock <= A.t[next].n);
-        }
+
+    int ahead = 0;   // tensor of the tile whose copies are issued
+    auto issue = [&](int q, Stage& s) {
+        if (q < total) {
+            ahead = tensor_of(A, q, ahead);
+            const AdamWTensor& T = A.t[ahead];
+            const uint32_t start = (uint32_t)(q - A.first[ahead]) * kTile;
+            if (T.aligned && start + kTile <= T.n) {
+                const float* p = T.p + start + t * 4;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const f32x2 gs = mul2(g.get(i), pair(A.grad_scale, A.grad_scale));
-            const f32x2 m1 = add2(mul2(m.get(i), pair(A.beta1, A.beta1)), mul2(gs, pair(A.one_minus_beta1, A.one_minus_beta1)));
-            const f32x2 v1 = add2(mul2(v.get(i), pair(A.beta2, A.beta2)), mul2(mul2(gs, pair(A.one_minus_beta2, A.one_minus_beta2)), gs));
-            m.set(i, m1);
-            v.set(i, v1);
-            // The moments are rounded step by step, since their codes depend on it; the step itself takes the fast root and reciprocal, which are off by 2^-23 of it
-            // (exact ones: two thirds more instructions). A denominator is zero or normal: the root of the smallest number is 2^-74.5.
-            float a, b;
-            unpair(add2(mul2(pair(fast_root(v.x[2 * i]), fast_root(v.x[2 * i + 1])), pair(A.bc2_sqrt_rcp, A.bc2_sqrt_rcp)), pair(A.eps, A.eps)), a, b);
-            const f32x2 step = mul2(mul2(m1, pair(T.step_size, T.step_size)), pair(fast_reciprocal(a), fast_reciprocal(b)));
-            p.set(i, sub2(mul2(p.get(i), pair(T.decay, T.decay)), step));
+                for (int k = 0; k < kBlocks; ++k) copy16(&s.p[k * kRow + t * 4], p + k * kRow);
+                if (T.grad_dtype == LFS_F32) {
+                    const float* g = static_cast<const float*>(T.g) + start + t * 4;
+#pragma unroll
+                    for (int k = 0; k < kBlocks; ++k) copy16(&s.g[k * kRow + t * 4], g + k * kRow);
+                } else copy16(&s.g[t * 4], static_cast<const uint16_t*>(T.g) + start + t * 8);
+                if (t < kTile / 16) copy16(&s.m[t * 16], static_cast<const uint8_t*>(T.m) + start + t * 16);
+                else copy16(&s.v[(t - kTile / 16) * 16], static_cast<const uint8_t*>(T.v) + start + (t - kTile / 16) * 16);
+                constexpr int kScales = kTile / kAdamWBlock / 4;
+                if (t < kScales) copy16(&s.ms[t * 4], T.ms + start / kAdamWBlock + t * 4);
+                else if (t < 2 * kScales) copy16(&s.vs[(t - kScales) * 4], T.vs + start / kAdamWBlock + (t - kScales) * 4);
+            }
         }
-        store4(T.p, e, T.n, whole, p);
-        if constexpr (BITS == 8) {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) issue(blockIdx.x + k * gridDim.x, stages[k]);
+    int now = 0, stage = 0;
+    for (int q = blockIdx.x; q < total; q += gridDim.x) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncthreads();   // everybody's copies of this tile are there, and everybody is done with the stage that is filled next
+        issue(q + (kStages - 1) * gridDim.x, stages[stage == 0 ? kStages - 1 : stage - 1]);
+        const Stage& s = stages[stage];
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        now = tensor_of(A, q, now);
+        const AdamWTensor& T = A.t[now];
+        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, A.bc2_sqrt_rcp, A.eps, T.step_size, T.decay};
+        const uint32_t tile = (uint32_t)(q - A.first[now]) * kTile;
+        if (!(T.aligned && tile + kTile <= T.n)) {
+            for (uint32_t start = tile + warp * kAdamWBlock; start < min(tile + kTile, T.n); start += kRow) single_block<8>(T, start, lane, S, A.offset_m, A.offset_v);
+            continue;
+        }
+        const uint32_t e0 = tile + t * 4;
+        const int dtype = T.grad_dtype;
+        float* const p_out = T.p + e0;
+        uint8_t *const m_out = static_cast<uint8_t*>(T.m) + e0, *const v_out = static_cast<uint8_t*>(T.v) + e0;
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            const int i = k * kRow + t * 4;
+            Block4 p = load4(s.p, i, 0, true), g, m, v;
+            if (dtype == LFS_F32) g = load4(s.g, i, 0, true);
+            else {
+                const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(s.g) + i);
+                g = {half_bits(w.x & 0xFFFFu, dtype), half_bits(w.x >> 16, dtype), half_bits(w.y & 0xFFFFu, dtype), half_bits(w.y >> 16, dtype)};
+            }
+            m = decode_m(load4(s.m, i, 0, true), s.ms[k * kWarps + warp]);
+            v = decode_v(load4(s.v, i, 0, true), s.vs[k * kWarps + warp]);
+            update(p, m, v, g, S);
+            store4(p_out, k * kRow, 0, true, p);
             float ms, vs;
-            if (!whole)   // what lies behind the tensor's end has no part in the scale
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (e + i >= T.n) m.x[i] = v.x[i] = 0.0f;
-            const uint32_t mc = encode4<false>(m, (uint32_t)e, A.offset_m, false, &ms);
-            const uint32_t vc = encode4<true>(v, (uint32_t)e, A.offset_v, false, &vs);
-            store4(static_cast<uint8_t*>(T.m), e, T.n, whole, mc);
-            store4(static_cast<uint8_t*>(T.v), e, T.n, whole, vc);
-            if (lane == 0) { T.ms[at / kAdamWBlock] = ms; T.vs[at / kAdamWBlock] = vs; }
-        } else {
-            store4(static_cast<float*>(T.m), e, T.n, whole, m);
-            store4(static_cast<float*>(T.v), e, T.n, whole, v);
+            const uint32_t e = T.before + e0 + k * kRow;
+            *reinterpret_cast<uint32_t*>(m_out + k * kRow) = encode_block<false>(m, e, A.offset_m, false, &ms);
+            *reinterpret_cast<uint32_t*>(v_out + k * kRow) = encode_block<true>(v, e, A.offset_v, false, &vs);
+            if (lane == 0) {
+                T.ms[tile / kAdamWBlock + k * kWarps + warp] = ms;
+                T.vs[tile / kAdamWBlock + k * kWarps + warp] = vs;
+            }
         }
-        if (!more) return;
+    }
+}
+
+// Moments in 32 bits: nothing but memory. A tile is a block to a warp, and the next one's loads are under way while it is computed.
+template <int CAP>
+__global__ void __launch_bounds__(kThreads, kCtas32) adamw32_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x;
+    const int total = A.first[A.n];
+    float4 p4, m4, v4;
+    uint4 g4;
+    int ahead = 0;
+    auto load = [&](int q) {
+        if (q >= total) return;
+        ahead = tensor_of(A, q, ahead);
+        const AdamWTensor& T = A.t[ahead];
+        const uint32_t tile = (uint32_t)(q - A.first[ahead]) * kRow, e = tile + t * 4;
+        if (!(T.aligned && tile + kRow <= T.n)) return;
+        p4 = *reinterpret_cast<const float4*>(T.p + e);
+        m4 = *reinterpret_cast<const float4*>(static_cast<const float*>(T.m) + e);
+        v4 = *reinterpret_cast<const float4*>(static_cast<const float*>(T.v) + e);
+        if (T.grad_dtype == LFS_F32) g4 = *reinterpret_cast<const uint4*>(static_cast<const float*>(T.g) + e);
+        else {
+            const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(T.g) + e);
+            g4 = make_uint4(w.x, w.y, 0, 0);
+        }
+    };
+    int now = 0;
+    load(blockIdx.x);
+    for (int q = blockIdx.x; q < total; q += gridDim.x) {
+        now = tensor_of(A, q, now);
+        const AdamWTensor& T = A.t[now];
+        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, A.bc2_sqrt_rcp, A.eps, T.step_size, T.decay};
+        const uint32_t tile = (uint32_t)(q - A.first[now]) * kRow, e = tile + t * 4;
+        const bool whole = T.aligned && tile + kRow <= T.n;
+        Block4 p{{p4.x, p4.y, p4.z, p4.w}}, m{{m4.x, m4.y, m4.z, m4.w}}, v{{v4.x, v4.y, v4.z, v4.w}}, g;
+        if (T.grad_dtype == LFS_F32) g = {__uint_as_float(g4.x), __uint_as_float(g4.y), __uint_as_float(g4.z), __uint_as_float(g4.w)};
+        else g = {half_bits(g4.x & 0xFFFFu, T.grad_dtype), half_bits(g4.x >> 16, T.grad_dtype), half_bits(g4.y & 0xFFFFu, T.grad_dtype), half_bits(g4.y >> 16, T.grad_dtype)};
+        load(q + gridDim.x);
+        if (whole) {
+            update(p, m, v, g, S);
+            store4(T.p, e, 0, true, p);
+            store4(static_cast<float*>(T.m), e, 0, true, m);
+            store4(static_cast<float*>(T.v), e, 0, true, v);
+        } else if (tile + warp * kAdamWBlock < T.n) single_block<32>(T, tile + warp * kAdamWBlock, lane, S, A.offset_m, A.offset_v);
     }
 }
 
@@ -302,7 +423,7 @@ __global__ void __launch_bounds__(256) adamw_encode_kernel(int64_t n, int64_t bl
         const bool whole = aligned && (b + 1) * kAdamWBlock <= n;
         const Block4 x = load4(values, e, n, whole);
         float scale;
-        const uint32_t c = second ? encode4<true>(x, 0, 0, true, &scale) : encode4<false>(x, 0, 0, true, &scale);
+        const uint32_t c = second ? encode_block<true>(x, 0, 0, true, &scale) : encode_block<false>(x, 0, 0, true, &scale);
         store4(codes, e, n, whole, c);
         if (lane == 0) scales[b] = scale;
     }
@@ -319,63 +440,92 @@ __global__ void __launch_bounds__(256) adamw_decode_kernel(int64_t n, int64_t bl
     }
 }
 
-// One launch over the tensors of one kind of moments (every tensor of a list, or those that are left when the other kind has been taken out).
+struct Host {
+    double beta1, beta2, eps;
+    int64_t step_count;
+    float grad_scale;
+    cudaStream_t st;
+};
+// One launch over pieces of tensors with the same kind of moments.
 template <int CAP, int BITS>
-int launch_adamw(int count, const lfs_adamw_tensor* const* tensors, double beta1, double beta2, double eps, int64_t step_count, float grad_scale, cudaStream_t st) {
+int launch_adamw(int count, const AdamWTensor* pieces, const Host& h) {
     static_assert(sizeof(AdamWArgs<CAP>) <= 32764, "kernel arguments");
-    // the same host arithmetic as lfs_adam_step_segments
-    const double bc1 = 1.0 / (1.0 - std::pow(beta1, (double)step_count));
-    const double bc2 = 1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step_count));
+    constexpr int kShared = kStages * (int)sizeof(Stage);
+    if (BITS == 8) {
+        // once per device, and again where it failed
+        static std::atomic<uint64_t> asked{0};
+        int device = 0;
+        if (cudaGetDevice(&device) != cudaSuccess || device > 63 || !(asked.load() >> device & 1)) {
+            if (cudaFuncSetAttribute(adamw8_kernel<CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess) return check_launch("adamw");
+            if (device < 64) asked.fetch_or((uint64_t)1 << device);
+        }
+    }
+    constexpr int kElements = BITS == 8 ? kTile : kRow;   // of a tile
     AdamWArgs<CAP> A;
-    int64_t blocks = 0;
+    int64_t tiles = 0;
     A.n = count;
     A.first[0] = 0;
     for (int k = 0; k < count; ++k) {
-        const lfs_adamw_tensor& t = *tensors[k];
-        AdamWTensor& o = A.t[k];
-        o.p = t.param; o.g = t.grad; o.m = t.exp_avg; o.v = t.exp_avg_sq; o.ms = t.exp_avg_scale; o.vs = t.exp_avg_sq_scale;
-        o.n = t.n;
-        o.step_size = (float)((double)t.lr * bc1);
-        o.decay = (float)(1.0 - (double)t.lr * (double)t.weight_decay);
-        o.grad_dtype = t.grad_dtype;
-        const uintptr_t moment = BITS == 8 ? 4 : 16;
-        o.aligned = aligned_by(t.param, 16) && aligned_by(t.grad, 4 * dtype_bytes(t.grad_dtype)) && aligned_by(t.exp_avg, moment) && aligned_by(t.exp_avg_sq, moment);
-        blocks += (t.n + kAdamWBlock - 1) / kAdamWBlock;
-        if (blocks >= (int64_t)1 << 30) {
-            set_error("lfs_adamw_step_tensors: more than 2^37 elements in one launch");
-            return LFS_EINVAL;
-        }
-        A.first[k + 1] = (int32_t)blocks;
+        A.t[k] = pieces[k];
+        tiles += (pieces[k].n + kElements - 1) / kElements;   // 2^20 at the most
+        A.first[k + 1] = (int32_t)tiles;
     }
-    A.beta1 = (float)beta1; A.beta2 = (float)beta2;
-    A.one_minus_beta1 = (float)(1.0 - beta1); A.one_minus_beta2 = (float)(1.0 - beta2);
-    A.eps = (float)eps; A.bc2_sqrt_rcp = (float)bc2; A.grad_scale = grad_scale;
-    A.offset_m = (uint32_t)step_count * kGolden;
-    A.offset_v = (uint32_t)step_count * kPlastic;
-    LFS_TIMED("adamw", st);
-    adamw_kernel<CAP, BITS><<<grid_for(blocks, 8, BITS == 8 ? kCtas8 : kCtas32), 256, 0, st>>>(A);
+    A.beta1 = (float)h.beta1; A.beta2 = (float)h.beta2;
+    A.one_minus_beta1 = (float)(1.0 - h.beta1); A.one_minus_beta2 = (float)(1.0 - h.beta2);
+    A.eps = (float)h.eps; A.bc2_sqrt_rcp = (float)(1.0 / std::sqrt(1.0 - std::pow(h.beta2, (double)h.step_count))); A.grad_scale = h.grad_scale;
+    A.offset_m = (uint32_t)h.step_count * kGolden;
+    A.offset_v = (uint32_t)h.step_count * kPlastic;
+    LFS_TIMED("adamw", h.st);
+    // With 32 tiles to a CTA and more, three CTAs per SM: us for 0.5, 1, 2 and 3 M Gaussians at SH degree 3 with four 83, 165, 327 and 487, with three 84, 162, 319 and 475; 30 k and 120 k (degree 3) 9.7 and
+    // 26.8, 10.4 and 28.0. (Moments in 32 bits: 1 M in 295, 257 and 304 with four, three and two.)
+    if (BITS == 8) adamw8_kernel<CAP><<<grid_for(tiles, 1, tiles >= 32ll * kCtas8 * num_sms() ? kCtas8 - 1 : kCtas8), kThreads, kShared, h.st>>>(A);
+    else adamw32_kernel<CAP><<<grid_for(tiles, 1, kCtas32), kThreads, 0, h.st>>>(A);
     return check_launch("adamw");
 }
 template <int BITS>
-int launch_adamw_kind(int n_tensors, const lfs_adamw_tensor* tensors, double beta1, double beta2, double eps, int64_t step_count, float grad_scale, cudaStream_t st) {
-    const lfs_adamw_tensor* some[kAdamWMany];
-    for (int k = 0; k < n_tensors;) {
-        int count = 0;
-        for (; k < n_tensors && count < kAdamWMany; ++k)
-            if (tensors[k].n > 0 && (tensors[k].exp_avg_scale != nullptr) == (BITS == 8)) some[count++] = tensors + k;
-        if (count == 0) continue;
-        const int rc = (count <= kAdamWFew ? launch_adamw<kAdamWFew, BITS> : launch_adamw<kAdamWMany, BITS>)(count, some, beta1, beta2, eps, step_count, grad_scale, st);
-        if (rc != LFS_OK) return rc;
+int launch_adamw_kind(int n_tensors, const lfs_adamw_tensor* tensors, const Host& h) {
+    AdamWTensor pieces[kAdamWMany];
+    int count = 0;
+    auto flush = [&] {
+        const int rc = count == 0 ? LFS_OK : count <= kAdamWFew ? launch_adamw<kAdamWFew, BITS>(count, pieces, h) : launch_adamw<kAdamWMany, BITS>(count, pieces, h);
+        count = 0;
+        return rc;
+    };
+    const double bc1 = 1.0 / (1.0 - std::pow(h.beta1, (double)h.step_count));   // the same host arithmetic as lfs_adam_step_segments
+    for (int k = 0; k < n_tensors; ++k) {
+        const lfs_adamw_tensor& t = tensors[k];
+        if ((t.exp_avg_scale != nullptr) != (BITS == 8)) continue;
+        const int grad_bytes = (int)dtype_bytes(t.grad_dtype), moment_bytes = BITS / 8;
+        for (int64_t at = 0; at < t.n; at += kPiece) {
+            if (count == kAdamWMany) {
+                const int rc = flush();
+                if (rc != LFS_OK) return rc;
+            }
+            AdamWTensor& o = pieces[count++];
+            o.p = t.param + at;
+            o.g = static_cast<const char*>(t.grad) + at * grad_bytes;
+            o.m = static_cast<char*>(t.exp_avg) + at * moment_bytes;
+            o.v = static_cast<char*>(t.exp_avg_sq) + at * moment_bytes;
+            o.ms = BITS == 8 ? t.exp_avg_scale + at / kAdamWBlock : nullptr;
+            o.vs = BITS == 8 ? t.exp_avg_sq_scale + at / kAdamWBlock : nullptr;
+            o.n = (uint32_t)std::min(t.n - at, kPiece);
+            o.before = (uint32_t)at;
+            o.step_size = (float)((double)t.lr * bc1);
+            o.decay = (float)(1.0 - (double)t.lr * (double)t.weight_decay);
+            o.grad_dtype = t.grad_dtype;
+            o.aligned = aligned_by(o.p, 16) && aligned_by(o.g, 16) && aligned_by(o.m, 16) && aligned_by(o.v, 16) && aligned_by(o.ms, 16) && aligned_by(o.vs, 16);
+        }
     }
-    return LFS_OK;
+    return flush();
 }
 
 }  // namespace
 
 int launch_adamw_tensors(int n_tensors, const lfs_adamw_tensor* tensors, double beta1, double beta2, double eps, int64_t step_count, float grad_scale,
                          cudaStream_t st) {
-    const int rc = launch_adamw_kind<32>(n_tensors, tensors, beta1, beta2, eps, step_count, grad_scale, st);
-    return rc != LFS_OK ? rc : launch_adamw_kind<8>(n_tensors, tensors, beta1, beta2, eps, step_count, grad_scale, st);
+    const Host h{beta1, beta2, eps, step_count, grad_scale, st};
+    const int rc = launch_adamw_kind<32>(n_tensors, tensors, h);
+    return rc != LFS_OK ? rc : launch_adamw_kind<8>(n_tensors, tensors, h);
 }
 
 int launch_adamw_encode(int64_t n, const float* values, int second_moment, uint8_t* codes, float* scales, cudaStream_t st) {

@@ -131,7 +131,7 @@ def _check_betas(betas, eps):
 
 
 class AdamW:
-    """AdamW over a list of tensors, one launch per 384 of them (lfs_adamw_step_tensors): per-image codes, exposure matrices, grids,
+    """AdamW over a list of tensors, one launch per 424 of them (lfs_adamw_step_tensors): per-image codes, exposure matrices, grids,
     palettes, small networks. Parameters are contiguous float32, gradients contiguous float32, bfloat16 or float16 of the same number of elements, on one device.
 
     Parameters, gradients and moments are bound here and stay bound: a step reads the gradients that are in those buffers by then (torch: zero_grad(set_to_none=False)),
