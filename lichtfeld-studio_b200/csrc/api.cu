@@ -1100,7 +1100,7 @@ int lfs_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int
     LFS_REQUIRE(v_table && aligned_by(v_table, 4), "null or misaligned v_table");
     if (n > 0) {
         LFS_REQUIRE(v_out && order && sorted_rows && workspace, "null pointer");
-        LFS_REQUIRE(aligned_by(v_out, dtype_bytes(dtype)) && aligned_by(order, 4) && aligned_by(sorted_rows, 4) && aligned_by(workspace, 256), "misaligned pointer");
+        LFS_REQUIRE(aligned_by(v_out, dtype_bytes(dtype)) && aligned16(order) && aligned16(sorted_rows) && aligned_by(workspace, 256), "misaligned pointer");
         if (workspace_bytes < embedding_bwd_bytes(n, width)) { set_error("lfs_embedding_bwd: workspace too small"); return LFS_ECAPACITY; }
     }
     return launch_embedding_bwd(n, rows, width, v_out, dtype, order, sorted_rows, scale, accumulate, v_table, workspace, S(stream));

@@ -128,42 +128,54 @@ int fwd_type(int64_t n, int64_t rows, int width, const void* table, const void* 
 }
 
 // ---- order --------------------------------------------------------------------------------------------
-// Stable radix sort of (row, position) by the row, up to 9 bits of it a pass: a CTA counts its 4096 lookups by their digit, one CTA per digit turns the
-// counts into places, and the lookups go there. Lookups that name no row sort behind all others, as row `rows`.
-constexpr int kSortThreads = 256, kSortWarps = kSortThreads / 32, kSortItems = 16, kSortTile = kSortThreads * kSortItems, kDigitBits = 9, kDigits = 1 << kDigitBits;
+// Stable radix sort of (row, position) by the row, up to 9 bits of it a pass: a CTA counts its lookups by their digit, one CTA per digit turns the
+// counts into places, and the lookups go there. Up to 2048 lookups one CTA does all passes. Lookups that name no row sort behind all others, as row `rows`.
+constexpr int kSortThreads = 256, kSortWarps = kSortThreads / 32, kDigitBits = 9, kDigits = 1 << kDigitBits;
+// Lookups of a thread: few shorten the launches while there are not many tiles, more give fewer counts (one pass over 400 k lookups 16.6 us with four and 18.6 with eight, over 3 M 59 and 54).
+constexpr int kItemsFew = 4, kItemsMany = 8;
+constexpr int64_t kManyLookups = 1 << 20;
+constexpr int kSmallSort = 2048;   // of one CTA: 6 us, where the launches take 10 to 20
 
 struct SortPass {
     int64_t n;
     uint32_t rows;
-    int shift, digits;         // digits: their number, a power of two
+    int shift, bits;
     int tiles;
     const void* indices;       // first pass
     int index_bits;
     const int32_t *rows_in, *at_in;   // later passes
 };
+__device__ __forceinline__ uint32_t index_key(const void* indices, int index_bits, uint32_t rows, int64_t i) {
+    const int64_t r = index_bits == 32 ? (int64_t) static_cast<const int32_t*>(indices)[i] : static_cast<const int64_t*>(indices)[i];
+    return r >= 0 && r < (int64_t)rows ? (uint32_t)r : rows;
+}
 template <bool FIRST>
 __device__ __forceinline__ uint32_t sort_key(const SortPass& P, int64_t i) {
-    if (!FIRST) return (uint32_t)P.rows_in[i];
-    const int64_t r = P.index_bits == 32 ? (int64_t) static_cast<const int32_t*>(P.indices)[i] : static_cast<const int64_t*>(P.indices)[i];
-    return r >= 0 && r < (int64_t)P.rows ? (uint32_t)r : P.rows;
+    return FIRST ? index_key(P.indices, P.index_bits, P.rows, i) : (uint32_t)P.rows_in[i];
 }
 
-template <bool FIRST>
+template <bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass P, uint32_t* __restrict__ counts) {
-    __shared__ uint32_t count[kDigits];
-    for (int d = threadIdx.x; d < P.digits; d += kSortThreads) count[d] = 0;
+    __shared__ uint32_t count[kSortWarps / 2][kDigits];   // two warps share one: less waiting for a digit that many lookups have
+    const int digits = 1 << P.bits;
+    let_next_start();
+    for (int d = threadIdx.x; d < kSortWarps / 2 * kDigits; d += kSortThreads) (&count[0][0])[d] = 0;
+    wait_for_previous();
     __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * kSortTile;
-#pragma unroll 4
-    for (int k = 0; k < kSortItems; ++k) {
+    const int64_t first = (int64_t)blockIdx.x * (kSortThreads * ITEMS);
+    uint32_t* const mine = count[threadIdx.x >> 6];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
         const int64_t i = first + k * kSortThreads + threadIdx.x;
-        const bool in = i < P.n;
-        const uint32_t d = in ? (sort_key<FIRST>(P, i) >> P.shift) & (P.digits - 1) : kDigits;
-        const uint32_t same = __match_any_sync(0xffffffffu, d);   // one addition for all lanes of a digit
-        if (in && (int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&count[d], __popc(same));
+        if (i < P.n) atomicAdd(&mine[(sort_key<FIRST>(P, i) >> P.shift) & (digits - 1)], 1u);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < P.digits; d += kSortThreads) counts[(size_t)d * P.tiles + blockIdx.x] = count[d];
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWarps / 2; ++w) sum += count[w][d];
+        counts[(size_t)d * P.tiles + blockIdx.x] = sum;
+    }
 }
 
 // exclusive prefix of one value per thread over the block of kSortThreads; the total to all threads
@@ -191,6 +203,8 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* warp_sums
 // counts of one digit in all tiles -> exclusive prefix over the tiles, and the digit's total
 __global__ void __launch_bounds__(kSortThreads) sort_scan_kernel(int tiles, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
     __shared__ uint32_t warp_sums[kSortWarps];
+    let_next_start();
+    wait_for_previous();
     uint32_t* c = counts + (size_t)blockIdx.x * tiles;
     uint32_t carry = 0;
     for (int t0 = 0; t0 < tiles; t0 += kSortThreads) {
@@ -204,43 +218,44 @@ __global__ void __launch_bounds__(kSortThreads) sort_scan_kernel(int tiles, uint
     if (threadIdx.x == 0) totals[blockIdx.x] = carry;
 }
 
-template <bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortPass P, const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
-                                                                  int32_t* __restrict__ rows_out, int32_t* __restrict__ at_out) {
-    __shared__ uint32_t place[kSortWarps][kDigits];
-    __shared__ uint32_t warp_sums[kSortWarps];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int d = threadIdx.x; d < kSortWarps * kDigits; d += kSortThreads) (&place[0][0])[d] = 0;
-    __syncthreads();
-    // a warp takes 32 neighbouring lookups at a time, in their order; a lookup's rank among its warp's of the same digit
-    const int64_t first = (int64_t)blockIdx.x * kSortTile + warp * (32 * kSortItems);
-    uint32_t key[kSortItems], rank[kSortItems];
-    int32_t at[kSortItems];
+// A warp's ITEMS * 32 lookups, 32 neighbouring ones at a time, in their order: each one's rank among the warp's of its digit, which `count` adds up. The lanes of a digit are found by a vote for
+// each of its bits. (The instruction that compares all lanes takes as long as there are different values: 27 us instead of 21 for the three launches of a pass over 20 k lookups.)
+template <int ITEMS>
+__device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ITEMS], int there, uint32_t* count, uint32_t (&rank)[ITEMS]) {
+    const int lane = threadIdx.x & 31;
+    uint32_t same[ITEMS];
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const int64_t i = first + k * 32 + lane;
-        key[k] = i < P.n ? sort_key<FIRST>(P, i) : 0u;
-        at[k] = FIRST ? (int32_t)i : i < P.n ? P.at_in[i] : 0;
+    for (int k = 0; k < ITEMS; ++k) {
+        same[k] = __ballot_sync(0xffffffffu, k * 32 + lane < there);
+#pragma unroll
+        for (int b = 0; b < kDigitBits; ++b) {
+            const bool one = (digit[k] >> b) & 1;
+            const uint32_t votes = __ballot_sync(0xffffffffu, one);
+            same[k] &= one ? votes : ~votes;
+        }
     }
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const bool in = first + k * 32 + lane < P.n;
-        const uint32_t d = in ? (key[k] >> P.shift) & (P.digits - 1) : kDigits;
-        const uint32_t same = __match_any_sync(0xffffffffu, d);
-        rank[k] = in ? place[warp][d] + __popc(same & ((1u << lane) - 1)) : 0u;
+    for (int k = 0; k < ITEMS; ++k) {
+        const bool in = k * 32 + lane < there;
+        const uint32_t before = count[digit[k]], lower = same[k] & ((1u << lane) - 1);
+        rank[k] = before + __popc(lower);
         __syncwarp();
-        if (in && lane == __ffs(same) - 1) place[warp][d] += __popc(same);
+        if (in && !lower) count[digit[k]] = before + __popc(same[k]);
         __syncwarp();
     }
-    __syncthreads();
-    // where the digits start, where this tile's lookups of a digit start, and where each warp's
+}
+// From the warps' counts of every digit: where each warp's first lookup of a digit goes. totals: lookups of a digit in all tiles and where this tile's start among them, or null: this CTA's alone.
+__device__ __forceinline__ void digit_places(uint32_t (*place)[kDigits], int digits, const uint32_t* counts, int tiles, const uint32_t* totals, uint32_t* warp_sums) {
     uint32_t carry = 0;
-    for (int d0 = 0; d0 < P.digits; d0 += kSortThreads) {
+    for (int d0 = 0; d0 < digits; d0 += kSortThreads) {
         const int d = d0 + threadIdx.x;
-        uint32_t all;
-        const uint32_t before = block_prefix(d < P.digits ? totals[d] : 0u, warp_sums, &all);
-        if (d < P.digits) {
-            uint32_t next = carry + before + counts[(size_t)d * P.tiles + blockIdx.x];
+        uint32_t own = 0, all;
+        if (d < digits && !totals)
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) own += place[w][d];
+        const uint32_t before = block_prefix(d >= digits ? 0u : totals ? totals[d] : own, warp_sums, &all);
+        if (d < digits) {
+            uint32_t next = carry + before + (totals ? counts[(size_t)d * tiles + blockIdx.x] : 0u);
 #pragma unroll
             for (int w = 0; w < kSortWarps; ++w) {
                 const uint32_t c = place[w][d];
@@ -250,24 +265,105 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortPass P, co
         }
         carry += all;
     }
+}
+
+template <bool FIRST, int ITEMS>
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortPass P, const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
+                                                                  int32_t* __restrict__ rows_out, int32_t* __restrict__ at_out) {
+    __shared__ uint32_t place[kSortWarps][kDigits];
+    __shared__ uint32_t warp_sums[kSortWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << P.bits;
+    const int64_t first = (int64_t)blockIdx.x * (kSortThreads * ITEMS) + warp * (32 * ITEMS);
+    uint32_t key[ITEMS], digit[ITEMS], rank[ITEMS];
+    int32_t at[ITEMS];
+    let_next_start();
+    for (int d = threadIdx.x; d < kSortWarps * kDigits; d += kSortThreads) (&place[0][0])[d] = 0;
+    wait_for_previous();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int64_t i = first + k * 32 + lane;
+        key[k] = i < P.n ? sort_key<FIRST>(P, i) : 0u;
+        at[k] = FIRST ? (int32_t)i : i < P.n ? P.at_in[i] : 0;
+    }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
+    for (int k = 0; k < ITEMS; ++k) digit[k] = (key[k] >> P.shift) & (digits - 1);
+    warp_ranks<ITEMS>(digit, (int)max((int64_t)0, min(P.n - first, (int64_t)(32 * ITEMS))), place[warp], rank);
+    __syncthreads();
+    digit_places(place, digits, counts, P.tiles, totals, warp_sums);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
         if (first + k * 32 + lane < P.n) {
-            const uint32_t to = place[warp][(key[k] >> P.shift) & (P.digits - 1)] + rank[k];
+            const uint32_t to = place[warp][digit[k]] + rank[k];
             rows_out[to] = (int32_t)key[k];
             at_out[to] = at[k];
         }
     }
 }
 
-struct SortPlan { int bits, passes, digit_bits, tiles; };
+// All passes over up to 32 * kSortWarps * ITEMS lookups, by one CTA.
+template <int ITEMS>
+__global__ void __launch_bounds__(kSortThreads) sort_small_kernel(int n, uint32_t rows, const void* __restrict__ indices, int index_bits, int passes, int bits,
+                                                                  int32_t* __restrict__ rows_out, int32_t* __restrict__ at_out) {
+    __shared__ uint32_t place[kSortWarps][kDigits];
+    __shared__ uint32_t warp_sums[kSortWarps];
+    __shared__ uint32_t key_s[kSortThreads * ITEMS];
+    __shared__ uint16_t at_s[kSortThreads * ITEMS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << bits;
+    const int first = warp * (32 * ITEMS);
+    uint32_t key[ITEMS], digit[ITEMS], rank[ITEMS];
+    int32_t at[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = first + k * 32 + lane;
+        key[k] = i < n ? index_key(indices, index_bits, rows, i) : 0u;
+        at[k] = i;
+    }
+    for (int p = 0; p < passes; ++p) {
+        for (int d = threadIdx.x; d < kSortWarps * kDigits; d += kSortThreads) (&place[0][0])[d] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) digit[k] = (key[k] >> (p * bits)) & (digits - 1);
+        warp_ranks<ITEMS>(digit, max(0, min(n - first, 32 * ITEMS)), place[warp], rank);
+        __syncthreads();
+        digit_places(place, digits, nullptr, 1, nullptr, warp_sums);
+        __syncthreads();
+        const bool last = p + 1 == passes;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            if (first + k * 32 + lane < n) {
+                const uint32_t to = place[warp][digit[k]] + rank[k];
+                if (last) {
+                    rows_out[to] = (int32_t)key[k];
+                    at_out[to] = at[k];
+                } else {
+                    key_s[to] = key[k];
+                    at_s[to] = (uint16_t)at[k];
+                }
+            }
+        }
+        __syncthreads();
+        if (last) return;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int i = first + k * 32 + lane;
+            if (i < n) {
+                key[k] = key_s[i];
+                at[k] = at_s[i];
+            }
+        }
+    }
+}
+
+struct SortPlan { int bits, passes, digit_bits, items, tiles; };
 SortPlan sort_plan(int64_t n, int64_t rows) {
     SortPlan p{};
     while ((rows >> p.bits) != 0) ++p.bits;   // keys are 0 .. rows
     p.passes = (p.bits + kDigitBits - 1) / kDigitBits;
     p.digit_bits = (p.bits + p.passes - 1) / p.passes;
-    p.tiles = (int)((n + kSortTile - 1) / kSortTile);
+    p.items = n > kManyLookups ? kItemsMany : kItemsFew;
+    p.tiles = (int)((n + kSortThreads * p.items - 1) / (kSortThreads * p.items));
     return p;
 }
 struct SortWs {
@@ -295,13 +391,17 @@ SortWs carve_sort(int64_t n, const SortPlan& p, void* base) {
 }
 
 // ---- gradient -------------------------------------------------------------------------------------------
-// A CTA takes a stretch of the sorted lookups, and a group of lanes a part of that, a row of v_out at a time, T of them under way. A row of the table whose lookups
-// lie in one group's part is written from there. Otherwise the first group that has some adds the others' sums to its own: each leaves what belongs to a row begun before it in shared
-// memory. What crosses stretches is left in the workspace, [stretch][head, tail][width], for embedding_join_kernel. Rows without lookups are cleared before.
+// A CTA takes a stretch of the sorted lookups, and a group of lanes a part of that, a row of v_out at a time, T of them under way. The group's lanes fetch four lookups each,
+// and the next four while it works on these. A row of the table whose lookups lie in one group's part is written from there. Otherwise the first group that has some adds the others' sums to its
+// own: each leaves what belongs to a row begun before it in shared memory. What crosses stretches is left in the workspace, [stretch][head, tail][width], for embedding_join_kernel. Rows
+// without lookups are cleared before.
 //
 // Sums are held in two floats: a million gradients of one row lose nothing, and the result is the exact sum rounded once (but for ties), whatever the stretches. Sums in 64 bits
 // took 273 us for a million lookups of 45 columns where these took 84: 32-bit values become 64-bit ones at a small fraction of the rate that additions have.
-constexpr int kBwdThreads = 256, kStretch = 1024, kTileUnits = 128;
+constexpr int kBwdThreads = 256, kTileUnits = 128;
+constexpr int64_t kOwnClear = 32768;   // elements of a table that a single CTA clears itself (a launch less: 1.5 us)
+// CTAs per SM by the sums that a lane holds
+constexpr int bwd_ctas(int sums) { return sums <= 4 ? 3 : 2; }
 
 // A sum in two floats: every rounding of the first is exact in the second (Knuth's two-sum). Explicit roundings, so that none of it is simplified away.
 struct Sum {
@@ -352,33 +452,37 @@ struct Sums {
 };
 
 template <int DTYPE, int V, int C, int T>
-__global__ void __launch_bounds__(kBwdThreads) embedding_bwd_kernel(int64_t n, int64_t rows, int width, int log_group, int stretch,
-                                                                    const typename Element<DTYPE>::T* __restrict__ v_out, const int32_t* __restrict__ order,
-                                                                    const int32_t* __restrict__ sorted_rows, float scale, int accumulate,
+__global__ void __launch_bounds__(kBwdThreads, bwd_ctas(C * V)) embedding_bwd_kernel(int64_t n, int64_t rows, int width, int log_group, int share, int clear, const typename Element<DTYPE>::T* __restrict__ v_out,
+                                                                    const int32_t* __restrict__ order, const int32_t* __restrict__ sorted_rows, float scale, int accumulate,
                                                                     float* __restrict__ v_table, Sum* __restrict__ parts) {
     using In = Pack<DTYPE, V>;
-    __shared__ int2 lookup_s[kStretch + 2];   // row and position; [0] and the one behind the last belong to the neighbours
+    __shared__ __align__(16) int32_t row_s[4 * kBwdThreads], at_s[4 * kBwdThreads];
     __shared__ Sum head_s[C * V][kBwdThreads];
+    __shared__ int32_t first_row_s;
     __shared__ uint8_t from_before_s[kBwdThreads], ends_s[kBwdThreads];   // by group: it begins inside a row, and that row ends in it
-    __shared__ int total_s;
-    const int64_t first = (int64_t)blockIdx.x * stretch;
-    const int there = (int)min((int64_t)stretch, n - first);
-    if (threadIdx.x == 0) {
-        lookup_s[0].x = first > 0 ? sorted_rows[first - 1] : -1;
-        lookup_s[there + 1].x = first + there < n ? sorted_rows[first + there] : -1;
-        total_s = there;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < there; i += kBwdThreads) {
-        const int32_t r = sorted_rows[first + i];
-        lookup_s[i + 1] = make_int2(r, order[first + i]);
-        if (r >= rows) atomicMin(&total_s, i);   // lookups that name no row are the last ones
-    }
-    __syncthreads();
-    const int total = total_s;
     const int group = 1 << log_group, lane = threadIdx.x & (group - 1), g = threadIdx.x >> log_group, groups = kBwdThreads >> log_group;
     const int units = width / V, unit0 = blockIdx.y * kTileUnits + lane;
-    const int share = stretch / groups, begin = min(g * share, total), end = min(begin + share, total);
+    const int64_t first = (int64_t)blockIdx.x * share * groups;
+    const int total = (int)min((int64_t)share * groups, n - first);
+    const int begin = min(g * share, total), end = min(begin + share, total);
+    let_next_start();
+    for (int i = threadIdx.x; i < clear; i += kBwdThreads) v_table[i] = 0.0f;   // by the only CTA, before it writes a row
+    int4 next_row{}, next_at{};
+    auto fetch = [&](int t) {   // four lookups of this lane, from t + 4 lane on
+        const int64_t i = first + t + 4 * lane;
+        if (t + 4 * lane + 4 <= end) {
+            next_row = *reinterpret_cast<const int4*>(sorted_rows + i);
+            next_at = *reinterpret_cast<const int4*>(order + i);
+        } else if (t + 4 * lane < end) {
+            const int left = end - t - 4 * lane;
+            next_row.x = sorted_rows[i];
+            next_at.x = order[i];
+            if (left > 1) { next_row.y = sorted_rows[i + 1]; next_at.y = order[i + 1]; }
+            if (left > 2) { next_row.z = sorted_rows[i + 2]; next_at.z = order[i + 2]; }
+        }
+    };
+    fetch(begin);
+    const int32_t before = begin < end && first + begin > 0 ? sorted_rows[first + begin - 1] : -1, after = begin < end && first + end < n ? sorted_rows[first + end] : -1;
     // lanes behind the last column read it again and write nothing
     const In* column[C];
 #pragma unroll
@@ -389,6 +493,7 @@ __global__ void __launch_bounds__(kBwdThreads) embedding_bwd_kernel(int64_t n, i
         for (int i = 0; i < C * V; ++i) head_s[i][threadIdx.x] = acc.get(i);
     };
     auto write_row = [&](int32_t row) {
+        if (row >= rows) return;
 #pragma unroll
         for (int k = 0; k < C; ++k) {
             const int u = unit0 + (k << log_group);
@@ -401,49 +506,63 @@ __global__ void __launch_bounds__(kBwdThreads) embedding_bwd_kernel(int64_t n, i
     };
     acc.clear();
     int32_t row = -1;
-    bool head = false, tail = false;
+    bool head = false, tail = false, from_before = false;
+    const int32_t *const my_rows = row_s + 4 * group * g, *const my_at = at_s + 4 * group * g;
+    auto take = [&](int t, auto count) {
+        constexpr int N = decltype(count)::value;
+        In x[N][C];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t at = (int64_t)my_at[t + i] * units;
+#pragma unroll
+            for (int k = 0; k < C; ++k) x[i][k] = column[k][at];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int32_t r = my_rows[t + i];
+            if (r != row) {
+                if (head) keep_head();
+                else write_row(row);
+                head = false;
+                acc.clear();
+                row = r;
+            }
+            float v[C * V];
+#pragma unroll
+            for (int k = 0; k < C; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[k * V + j] = Element<DTYPE>::from(x[i][k].x[j]);
+            acc.add(v);
+        }
+    };
+    if (clear) __syncthreads();
+    // every group of a warp goes round as often as the others
+    for (int t = 0; t < share; t += 4 * group) {
+        __syncwarp();
+        reinterpret_cast<int4*>(row_s)[threadIdx.x] = next_row;
+        reinterpret_cast<int4*>(at_s)[threadIdx.x] = next_at;
+        __syncwarp();
+        fetch(begin + t + 4 * group);
+        const int count = min(4 * group, end - begin - t);
+        if (count <= 0) continue;
+        if (t == 0) {
+            row = my_rows[0];
+            head = from_before = before == row;
+            if (g == 0 && lane == 0) first_row_s = row;
+        }
+        if (my_rows[0] >= rows && row >= rows) continue;   // lookups that name no row are the last ones
+        int i = 0;
+        for (; i + T <= count; i += T) take(i, Constant<int, T>{});
+        for (; i < count; ++i) take(i, Constant<int, 1>{});
+    }
     if (begin < end) {
-        row = lookup_s[begin + 1].x;
-        const bool from_before = lookup_s[begin].x == row;
-        head = from_before;
-        auto take = [&](int t, auto count) {
-            constexpr int N = decltype(count)::value;
-            int32_t r[N];
-            In x[N][C];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int2 l = lookup_s[t + i + 1];
-                r[i] = l.x;
-#pragma unroll
-                for (int k = 0; k < C; ++k) x[i][k] = column[k][(int64_t)l.y * units];
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if (r[i] != row) {
-                    if (head) keep_head();
-                    else write_row(row);
-                    head = false;
-                    acc.clear();
-                    row = r[i];
-                }
-                float v[C * V];
-#pragma unroll
-                for (int k = 0; k < C; ++k)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) v[k * V + j] = Element<DTYPE>::from(x[i][k].x[j]);
-                acc.add(v);
-            }
-        };
-        int t = begin;
-        for (; t + T <= end; t += T) take(t, Constant<int, T>{});
-        for (; t < end; ++t) take(t, Constant<int, 1>{});
-        const bool goes_on = lookup_s[end + 1].x == row;
+        const bool goes_on = after == row;
         if (lane == 0) {
             from_before_s[g] = from_before;
             ends_s[g] = !head || !goes_on;
         }
         if (head) keep_head();
-        else if (goes_on) tail = true;
+        else if (goes_on) tail = row < rows;
         else write_row(row);
     }
     __syncthreads();
@@ -472,7 +591,7 @@ __global__ void __launch_bounds__(kBwdThreads) embedding_bwd_kernel(int64_t n, i
         }
     };
     if (tail) join(row, false);
-    if (g == 0 && begin < end && from_before_s[0]) join(lookup_s[1].x, true);
+    if (g == 0 && begin < end && from_before && first_row_s < rows) join(first_row_s, true);
 }
 
 // The rows that lie in several stretches: the one that has a row's tail adds the heads of those that follow. A CTA per stretch; its threads are columns by slices of the heads.
@@ -481,6 +600,7 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int64_t n,
                                                                       float scale, int accumulate, const Sum* __restrict__ parts, float* __restrict__ v_table) {
     __shared__ Sum sum_s[kJoinThreads];
     __shared__ int next_s;
+    wait_for_previous();
     const int c = blockIdx.x;
     const int64_t first = (int64_t)c * stretch, end = min(first + stretch, n);
     const int32_t row = sorted_rows[end - 1];
@@ -517,7 +637,15 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int64_t n,
     }
 }
 
-int64_t bwd_stretches(int64_t n) { return (n + kStretch - 1) / kStretch; }
+// lookups of a group and number of stretches: all CTAs at once where there are that many lookups, and 4 a lane at least
+struct Cut { int share; int64_t stretches; };
+Cut bwd_cut(int64_t n, int log_group, int ctas, int column_tiles) {
+    const int64_t groups = kBwdThreads >> log_group, slots = max(1, num_sms() * ctas / column_tiles), step = 4 << log_group;
+    const int64_t share = max(step, ((n + slots * groups - 1) / (slots * groups) + 3) / 4 * 4);
+    return {(int)share, (n + share * groups - 1) / (share * groups)};
+}
+// the most stretches that a call may have, for any alignment
+int64_t bwd_stretches(int64_t n) { return (n + 4 * kBwdThreads - 1) / (4 * kBwdThreads); }
 
 struct Bwd {
     int64_t n, rows;
@@ -531,18 +659,28 @@ struct Bwd {
 };
 template <int DTYPE, int V, int C>
 int bwd(const Bwd& b) {
-    constexpr int T = C * V <= 4 ? 8 : C * V <= 8 ? 4 : 2;
-    const dim3 grid((unsigned)bwd_stretches(b.n), (unsigned)((b.width / V + kTileUnits - 1) / kTileUnits));
-    embedding_bwd_kernel<DTYPE, V, C, T><<<grid, kBwdThreads, 0, b.st>>>(b.n, b.rows, b.width, b.log_group, kStretch, static_cast<const typename Element<DTYPE>::T*>(b.v_out),
-                                                                         b.order, b.sorted_rows, b.scale, b.accumulate, b.v_table, b.parts);
-    return check_launch("embedding_bwd");
+    constexpr int T = C * V <= 4 ? 4 : C * V <= 8 ? 4 : 2;
+    const int column_tiles = (b.width / V + kTileUnits - 1) / kTileUnits;
+    const Cut cut = bwd_cut(b.n, b.log_group, bwd_ctas(C * V), column_tiles);
+    const bool alone = cut.stretches == 1 && column_tiles == 1 && b.rows * b.width <= kOwnClear;
+    if (!b.accumulate && !alone && cudaMemsetAsync(b.v_table, 0, (size_t)b.rows * b.width * sizeof(float), b.st) != cudaSuccess) {
+        set_error("lfs_embedding_bwd: memset failed");
+        return LFS_ECUDA;
+    }
+    embedding_bwd_kernel<DTYPE, V, C, T><<<dim3((unsigned)cut.stretches, (unsigned)column_tiles), kBwdThreads, 0, b.st>>>(
+        b.n, b.rows, b.width, b.log_group, cut.share, alone && !b.accumulate ? (int)(b.rows * b.width) : 0, static_cast<const typename Element<DTYPE>::T*>(b.v_out), b.order, b.sorted_rows, b.scale, b.accumulate, b.v_table, b.parts);
+    const int rc = check_launch("embedding_bwd");
+    if (rc != LFS_OK || cut.stretches == 1) return rc;
+    launch_beside(embedding_join_kernel, (int)cut.stretches, kJoinThreads, 0, b.st, b.n, b.rows, b.width, cut.share * (kBwdThreads >> b.log_group), (int)cut.stretches, b.sorted_rows, b.scale,
+                  b.accumulate, (const Sum*)b.parts, b.v_table);
+    return check_launch("embedding_join");
 }
 template <int DTYPE, int V>
 int bwd_units(Bwd b) {
     // lanes of a group times units of a lane: as few as cover the row, and then as many lanes as that leaves
     const int units = min(b.width / V, kTileUnits);
     int best = 1 << 30, per_lane = 1;
-    for (int log_group = 5; log_group >= 0; --log_group) {
+    for (int log_group = 5; log_group >= 1; --log_group) {
         const int c = (units + (1 << log_group) - 1) >> log_group;
         if (c <= 4 && (c << log_group) < best) { best = c << log_group; b.log_group = log_group; per_lane = c; }
     }
@@ -570,27 +708,39 @@ int launch_embedding_fwd(int64_t n, int64_t rows, int width, const void* table, 
 
 size_t embedding_sort_bytes(int64_t n, int64_t rows) { return carve_sort(n, sort_plan(n, rows), nullptr).bytes; }
 
+// Each launch of a pass begins while the one before it ends, and waits for it before it reads.
+template <bool FIRST, int ITEMS>
+static void launch_sort_pass(const SortPass& P, const SortWs& w, int32_t* rows_out, int32_t* at_out, cudaStream_t st) {
+    if (FIRST) launch(sort_count_kernel<FIRST, ITEMS>, P.tiles, kSortThreads, 0, st, P, w.counts);
+    else launch_beside(sort_count_kernel<FIRST, ITEMS>, P.tiles, kSortThreads, 0, st, P, w.counts);
+    launch_beside(sort_scan_kernel, 1 << P.bits, kSortThreads, 0, st, P.tiles, w.counts, w.totals);
+    launch_beside(sort_place_kernel<FIRST, ITEMS>, P.tiles, kSortThreads, 0, st, P, (const uint32_t*)w.counts, (const uint32_t*)w.totals, rows_out, at_out);
+}
+
 int launch_embedding_sort(int64_t n, int64_t rows, const void* indices, int index_bits, int32_t* order, int32_t* sorted_rows, void* workspace, cudaStream_t st) {
     if (n == 0) return LFS_OK;
     LFS_TIMED("embedding_sort", st);
     const SortPlan p = sort_plan(n, rows);
+    if (n <= kSmallSort) {
+        (n <= kSortThreads ? sort_small_kernel<1> : n <= 4 * kSortThreads ? sort_small_kernel<4> : sort_small_kernel<kSmallSort / kSortThreads>)<<<1, kSortThreads, 0, st>>>(
+            (int)n, (uint32_t)rows, indices, index_bits, p.passes, p.digit_bits, sorted_rows, order);
+        return check_launch("embedding_sort");
+    }
     const SortWs w = carve_sort(n, p, workspace);
     for (int k = 0; k < p.passes; ++k) {
-        const bool first = k == 0, mine = (p.passes - 1 - k) % 2 == 0;   // the last pass writes the caller's arrays
+        const bool mine = (p.passes - 1 - k) % 2 == 0;   // the last pass writes the caller's arrays
         SortPass P{};
         P.n = n; P.rows = (uint32_t)rows;
         P.shift = k * p.digit_bits;
-        P.digits = 1 << p.digit_bits;
+        P.bits = p.digit_bits;
         P.tiles = p.tiles;
         P.indices = indices; P.index_bits = index_bits;
         P.rows_in = mine ? w.rows : sorted_rows;
         P.at_in = mine ? w.at : order;
         int32_t *rows_out = mine ? sorted_rows : w.rows, *at_out = mine ? order : w.at;
-        if (first) sort_count_kernel<true><<<p.tiles, kSortThreads, 0, st>>>(P, w.counts);
-        else sort_count_kernel<false><<<p.tiles, kSortThreads, 0, st>>>(P, w.counts);
-        sort_scan_kernel<<<P.digits, kSortThreads, 0, st>>>(p.tiles, w.counts, w.totals);
-        if (first) sort_place_kernel<true><<<p.tiles, kSortThreads, 0, st>>>(P, w.counts, w.totals, rows_out, at_out);
-        else sort_place_kernel<false><<<p.tiles, kSortThreads, 0, st>>>(P, w.counts, w.totals, rows_out, at_out);
+        const bool few = p.items == kItemsFew;
+        (k == 0 ? few ? launch_sort_pass<true, kItemsFew> : launch_sort_pass<true, kItemsMany>
+                : few ? launch_sort_pass<false, kItemsFew> : launch_sort_pass<false, kItemsMany>)(P, w, rows_out, at_out, st);
     }
     return check_launch("embedding_sort");
 }
@@ -600,17 +750,15 @@ size_t embedding_bwd_bytes(int64_t n, int width) { return (size_t)bwd_stretches(
 int launch_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, float scale,
                          int accumulate, float* v_table, void* workspace, cudaStream_t st) {
     LFS_TIMED("embedding_bwd", st);
-    if (!accumulate && cudaMemsetAsync(v_table, 0, (size_t)rows * width * sizeof(float), st) != cudaSuccess) {
-        set_error("lfs_embedding_bwd: memset failed");
-        return LFS_ECUDA;
+    if (n == 0) {
+        if (!accumulate && cudaMemsetAsync(v_table, 0, (size_t)rows * width * sizeof(float), st) != cudaSuccess) {
+            set_error("lfs_embedding_bwd: memset failed");
+            return LFS_ECUDA;
+        }
+        return LFS_OK;
     }
-    if (n == 0) return LFS_OK;
     const Bwd b{n, rows, width, 0, accumulate, v_out, order, sorted_rows, scale, v_table, static_cast<Sum*>(workspace), st};
-    const int rc = dtype == LFS_F32 ? bwd_type<LFS_F32>(b) : dtype == LFS_BF16 ? bwd_type<LFS_BF16>(b) : bwd_type<LFS_F16>(b);
-    const int64_t stretches = bwd_stretches(n);
-    if (rc != LFS_OK || stretches == 1) return rc;
-    embedding_join_kernel<<<(unsigned)stretches, kJoinThreads, 0, st>>>(n, rows, width, kStretch, (int)stretches, sorted_rows, b.scale, accumulate, b.parts, v_table);
-    return check_launch("embedding_join");
+    return dtype == LFS_F32 ? bwd_type<LFS_F32>(b) : dtype == LFS_BF16 ? bwd_type<LFS_BF16>(b) : bwd_type<LFS_F16>(b);
 }
 
 }  // namespace lfs

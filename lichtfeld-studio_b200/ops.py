@@ -357,7 +357,7 @@ def embedding_sort(indices, rows):
     rows, n, dev = int(rows), indices.numel(), indices.device
     if not 1 <= rows <= _MAX_ROWS or n > _MAX_ROWS:
         raise RuntimeError(f"bad sizes: {n} indices, {rows} rows")
-    order, sorted_rows = torch.empty((2, n), dtype=torch.int32, device=dev)
+    order, sorted_rows = (torch.empty(n, dtype=torch.int32, device=dev) for _ in range(2))
     if n:
         ws = _ws(capi.lib().lfs_embedding_sort_workspace_bytes(n, rows), dev)
         _call_on(dev, "lfs_embedding_sort", n, rows, ptr(indices), indices.element_size() * 8, ptr(order), ptr(sorted_rows), ptr(ws), ws.numel())
