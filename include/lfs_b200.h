@@ -462,7 +462,8 @@ int lfs_embedding_fwd(int64_t n, int64_t rows, int width, const void* table, int
                       float scale, void* out, int out_dtype, void* stream);
 
 /* The lookups in the order of their rows, ties by their position: sorted_rows [n] = the rows in ascending order (`rows` for
- * indices that name none), order [n] = their positions in `indices`. It can be kept for as long as the indices stay the same. n, rows < 2^31 - 1. */
+ * indices that name none), order [n] = their positions in `indices`. It can be kept for as long as the indices stay the same. n, rows < 2^31 - 1.
+ * A workspace of 0 bytes may be NULL (few lookups), here and in lfs_embedding_bwd. */
 size_t lfs_embedding_sort_workspace_bytes(int64_t n, int64_t rows);
 int lfs_embedding_sort(int64_t n, int64_t rows, const void* indices, int index_bits, int32_t* order, int32_t* sorted_rows,
                        void* workspace, size_t workspace_bytes, void* stream);

@@ -1081,7 +1081,7 @@ int lfs_embedding_sort(int64_t n, int64_t rows, const void* indices, int index_b
     if (rc != LFS_OK) return rc;
     LFS_REQUIRE(index_bits == 32 || index_bits == 64, "index_bits must be 32 or 64");
     if (n == 0) return LFS_OK;
-    LFS_REQUIRE(indices && order && sorted_rows && workspace, "null pointer");
+    LFS_REQUIRE(indices && order && sorted_rows && (workspace || embedding_sort_bytes(n, rows) == 0), "null pointer");
     LFS_REQUIRE(aligned_by(indices, (uintptr_t)index_bits / 8) && aligned_by(order, 4) && aligned_by(sorted_rows, 4) && aligned_by(workspace, 256), "misaligned pointer");
     if (workspace_bytes < embedding_sort_bytes(n, rows)) { set_error("lfs_embedding_sort: workspace too small"); return LFS_ECAPACITY; }
     return launch_embedding_sort(n, rows, indices, index_bits, order, sorted_rows, workspace, S(stream));
@@ -1099,7 +1099,7 @@ int lfs_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int
     LFS_REQUIRE(dtype_ok(dtype), "dtype must be LFS_F32, LFS_BF16 or LFS_F16");
     LFS_REQUIRE(v_table && aligned_by(v_table, 4), "null or misaligned v_table");
     if (n > 0) {
-        LFS_REQUIRE(v_out && order && sorted_rows && workspace, "null pointer");
+        LFS_REQUIRE(v_out && order && sorted_rows && (workspace || embedding_bwd_bytes(n, width) == 0), "null pointer");
         LFS_REQUIRE(aligned_by(v_out, dtype_bytes(dtype)) && aligned16(order) && aligned16(sorted_rows) && aligned_by(workspace, 256), "misaligned pointer");
         if (workspace_bytes < embedding_bwd_bytes(n, width)) { set_error("lfs_embedding_bwd: workspace too small"); return LFS_ECAPACITY; }
     }

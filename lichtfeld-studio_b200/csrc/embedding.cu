@@ -706,7 +706,7 @@ int launch_embedding_fwd(int64_t n, int64_t rows, int width, const void* table, 
                                 : fwd_type<LFS_F16, LFS_F16>(n, rows, width, table, indices, index_bits, scale, out, st);
 }
 
-size_t embedding_sort_bytes(int64_t n, int64_t rows) { return carve_sort(n, sort_plan(n, rows), nullptr).bytes; }
+size_t embedding_sort_bytes(int64_t n, int64_t rows) { return n <= kSmallSort ? 0 : carve_sort(n, sort_plan(n, rows), nullptr).bytes; }
 
 // Each launch of a pass begins while the one before it ends, and waits for it before it reads.
 template <bool FIRST, int ITEMS>
@@ -745,7 +745,7 @@ int launch_embedding_sort(int64_t n, int64_t rows, const void* indices, int inde
     return check_launch("embedding_sort");
 }
 
-size_t embedding_bwd_bytes(int64_t n, int width) { return (size_t)bwd_stretches(n) * 2 * width * sizeof(Sum); }
+size_t embedding_bwd_bytes(int64_t n, int width) { return bwd_stretches(n) <= 1 ? 0 : (size_t)bwd_stretches(n) * 2 * width * sizeof(Sum); }
 
 int launch_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, float scale,
                          int accumulate, float* v_table, void* workspace, cudaStream_t st) {

@@ -295,11 +295,12 @@ _MAX_ROWS = (1 << 31) - 2
 
 def _call_on(device, name, *args):
     """The call on the current stream of the tensors' device, which becomes the current one for it."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, _stream())
+    index = device.index
+    if index == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))   # what torch.cuda.current_stream().cuda_stream gives, without the 3 us of its object
     else:
-        with torch.cuda.device(device):
-            call(name, *args, _stream())
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _check_typed(t, name, dtypes, device=None):
@@ -315,77 +316,94 @@ def _check_typed(t, name, dtypes, device=None):
         raise RuntimeError(f"{name} must be a CUDA tensor")
 
 
+_INDICES = {torch.int32: 32, torch.int64: 64}
+
+
 def embedding_fwd(table, indices, scale=1.0, out_dtype=None, out=None):
     """scale * table[indices]: [*indices.shape, width] of the table's type or float32. table [rows, width] float32, bfloat16 or
     float16; indices int32 or int64 of any shape. An index below 0 or not below `rows` gives zeros. `out` receives the result
-    (contiguous, its element type is the out_dtype)."""
+    (contiguous, its element type is the out_dtype; it must not overlap the inputs)."""
     _check_typed(table, "table", _DTYPES)
+    device, dtype = table.device, table.dtype
     if table.dim() != 2 or not 1 <= table.shape[0] <= _MAX_ROWS or not 1 <= table.shape[1] <= capi.LFS_EMBEDDING_MAX_WIDTH:
         raise RuntimeError(f"table must be [rows, width] with at least one row and column, got {list(table.shape)}")
-    _check_typed(indices, "indices", (torch.int32, torch.int64), table.device)
+    _check_typed(indices, "indices", _INDICES, device)
     rows, width = table.shape
-    shape = (*indices.shape, width)
-    if indices.numel() > _MAX_ROWS:
+    n = indices.numel()
+    if n > _MAX_ROWS:
         raise RuntimeError("too many indices")
+    to = (out_dtype or dtype) if out is None else out.dtype
+    if to not in (dtype, torch.float32):
+        raise RuntimeError(f"out must be {dtype} or torch.float32, got {to}")
     if out is None:
-        dtype = out_dtype or table.dtype
+        out = torch.empty((*indices.shape, width), dtype=to, device=device)
     else:
-        dtype = out.dtype
-        if out_dtype not in (None, dtype) or out.numel() != indices.numel() * width:
-            raise RuntimeError(f"out must hold {indices.numel()} rows of {width} elements of the out_dtype")
-        _check_typed(out, "out", _DTYPES, table.device)
-    if dtype not in (table.dtype, torch.float32):
-        raise RuntimeError(f"out must be {table.dtype} or torch.float32, got {dtype}")
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=table.device)
-    if indices.numel():
-        _call_on(table.device, "lfs_embedding_fwd", indices.numel(), rows, width, ptr(table), _DTYPES[table.dtype], ptr(indices),
-                 indices.element_size() * 8, float(scale), ptr(out), _DTYPES[dtype])
+        if out_dtype not in (None, to) or out.numel() != n * width:
+            raise RuntimeError(f"out must hold {n} rows of {width} elements of the out_dtype")
+        _check_typed(out, "out", _DTYPES, device)
+    if n:
+        _call_on(device, "lfs_embedding_fwd", n, rows, width, table.data_ptr(), _DTYPES[dtype], indices.data_ptr(), _INDICES[indices.dtype], float(scale),
+                 out.data_ptr(), _DTYPES[to])
     return out
 
 
 class EmbeddingOrder:
-    """The lookups of one tensor of indices in the order of their rows (embedding_sort), for as many embedding_bwd as share it."""
+    """The lookups of one tensor of indices in the order of their rows (embedding_sort), for as many embedding_bwd as share it:
+    sorted_rows ascending (`rows` for indices that name no row) and order, their positions."""
 
-    def __init__(self, shape, rows, order, sorted_rows):
-        self.shape, self.rows, self.order, self.sorted_rows = shape, rows, order, sorted_rows
+    def __init__(self, shape, n, rows, buffer, stride):
+        self.shape, self.n, self.rows, self._buffer, self._stride = shape, n, rows, buffer, stride
+
+    @property
+    def order(self):
+        return self._buffer[: self.n]
+
+    @property
+    def sorted_rows(self):
+        return self._buffer[self._stride: self._stride + self.n]
 
 
 def embedding_sort(indices, rows):
     """The order that embedding_bwd goes by. Stable: lookups of one row stay in the order of their positions."""
-    _check_typed(indices, "indices", (torch.int32, torch.int64))
-    rows, n, dev = int(rows), indices.numel(), indices.device
+    _check_typed(indices, "indices", _INDICES)
+    rows, n, device = int(rows), indices.numel(), indices.device
     if not 1 <= rows <= _MAX_ROWS or n > _MAX_ROWS:
         raise RuntimeError(f"bad sizes: {n} indices, {rows} rows")
-    order, sorted_rows = (torch.empty(n, dtype=torch.int32, device=dev) for _ in range(2))
+    stride = (n + 63) // 64 * 64   # both halves are 256-byte aligned
+    buffer = torch.empty(2 * stride, dtype=torch.int32, device=device)
     if n:
-        ws = _ws(capi.lib().lfs_embedding_sort_workspace_bytes(n, rows), dev)
-        _call_on(dev, "lfs_embedding_sort", n, rows, ptr(indices), indices.element_size() * 8, ptr(order), ptr(sorted_rows), ptr(ws), ws.numel())
-    return EmbeddingOrder(indices.shape, rows, order, sorted_rows)
+        nbytes = capi.lib().lfs_embedding_sort_workspace_bytes(n, rows)
+        ws = _ws(nbytes, device) if nbytes else None
+        base = buffer.data_ptr()
+        _call_on(device, "lfs_embedding_sort", n, rows, indices.data_ptr(), _INDICES[indices.dtype], base, base + 4 * stride,
+                 None if ws is None else ws.data_ptr(), nbytes)
+    return EmbeddingOrder(indices.shape, n, rows, buffer, stride)
 
 
 def embedding_bwd(v_out, order, scale=1.0, out=None, accumulate=False):
     """Gradient of embedding_fwd with respect to the table: [rows, width] float32, scale times the sum of v_out over every row's
     lookups, zeros for rows without any. v_out [*indices.shape, width] float32, bfloat16 or float16. `out` receives it, or is added to with
-    `accumulate`. The same call gives the same bits."""
+    `accumulate` (it must not overlap v_out). The same call gives the same bits."""
     if not isinstance(order, EmbeddingOrder):
         raise RuntimeError("order must come from embedding_sort")
-    _check_typed(v_out, "v_out", _DTYPES, order.order.device)
-    n, rows = order.order.numel(), order.rows
+    device, n, rows = order._buffer.device, order.n, order.rows
+    _check_typed(v_out, "v_out", _DTYPES, device)
     if v_out.dim() < 1 or v_out.shape[:-1] != order.shape or not 1 <= v_out.shape[-1] <= capi.LFS_EMBEDDING_MAX_WIDTH:
         raise RuntimeError(f"v_out must be {[*order.shape, 'width']}, got {list(v_out.shape)}")
-    width, dev = v_out.shape[-1], v_out.device
+    width = v_out.shape[-1]
     if out is None:
         if accumulate:
             raise RuntimeError("accumulate needs an out to add to")
-        out = torch.empty((rows, width), dtype=torch.float32, device=dev)
+        out = torch.empty((rows, width), dtype=torch.float32, device=device)
     else:
-        _check_typed(out, "out", (torch.float32,), dev)
+        _check_typed(out, "out", (torch.float32,), device)
         if out.numel() != rows * width:
             raise RuntimeError(f"out must hold {rows} rows of {width} elements")
-    ws = _ws(capi.lib().lfs_embedding_bwd_workspace_bytes(n, width), dev)
-    _call_on(dev, "lfs_embedding_bwd", n, rows, width, ptr(v_out), _DTYPES[v_out.dtype], ptr(order.order), ptr(order.sorted_rows), float(scale),
-             1 if accumulate else 0, ptr(out), ptr(ws), ws.numel())
+    nbytes = capi.lib().lfs_embedding_bwd_workspace_bytes(n, width)
+    ws = _ws(nbytes, device) if nbytes else None
+    base = order._buffer.data_ptr()
+    _call_on(device, "lfs_embedding_bwd", n, rows, width, v_out.data_ptr(), _DTYPES[v_out.dtype], base, base + 4 * order._stride, float(scale),
+             1 if accumulate else 0, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 

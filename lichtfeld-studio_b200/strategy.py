@@ -161,7 +161,8 @@ class AdamW:
             m.check(p.numel(), self.device, f"moments[{i}]")
         self.lr, self.weight_decay = _each(lr, n, "lr"), _each(weight_decay, n, "weight_decay")
         self.step_count = 0
-        self._table = np.zeros(n, _TABLE)
+        self._table, self._rates = np.zeros(n, _TABLE), None
+        self._address = self._table.ctypes.data
         self._table["param"] = [p.data_ptr() for p in self.params]
         for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
             self._table[name] = [0 if getattr(m, name) is None else getattr(m, name).data_ptr() for m in self.moments]
@@ -191,8 +192,11 @@ class AdamW:
 
     def step(self, grad_scale: float = 1.0):
         """One update from the bound gradients, which grad_scale multiplies."""
-        self._table["lr"], self._table["weight_decay"] = self.lr, self.weight_decay
-        ops._call_on(self.device, "lfs_adamw_step_tensors", len(self._table), self._table.ctypes.data, self.betas[0], self.betas[1], self.eps,
+        rates = (list(self.lr), list(self.weight_decay))
+        if rates != self._rates:
+            self._table["lr"], self._table["weight_decay"] = rates
+            self._rates = rates
+        ops._call_on(self.device, "lfs_adamw_step_tensors", len(self._table), self._address, self.betas[0], self.betas[1], self.eps,
                      self.step_count + 1, float(grad_scale))
         self.step_count += 1
 

@@ -67,18 +67,20 @@ def test_embedding_calls_refuse(pkg):
                 dict(tt=3), dict(tt=0, ot=1), dict(tt=1, ot=2), dict(bits=16), dict(table=P + 2), dict(idx=P + 4, bits=64), dict(out=P + 1)):
         assert fwd(**bad) == einval, bad
     assert fwd(n=0, table=None, idx=None, out=None) == 0
-    size = l.lfs_embedding_sort_workspace_bytes(5, 3)
-    assert size > 0 and l.lfs_embedding_sort_workspace_bytes(5, 0) == 0
-    def sort(n=5, rows=3, idx=P, bits=32, order=P, srt=P, ws=P, size=size):
+    many = 100_000    # a few lookups need no workspace
+    size = l.lfs_embedding_sort_workspace_bytes(many, 3)
+    assert size > 0 and l.lfs_embedding_sort_workspace_bytes(5, 3) == l.lfs_embedding_sort_workspace_bytes(5, 0) == 0
+    def sort(n=many, rows=3, idx=P, bits=32, order=P, srt=P, ws=P, size=size):
         return l.lfs_embedding_sort(n, rows, idx, bits, order, srt, ws, size, None)
     for bad in (dict(n=-1), dict(rows=0), dict(idx=None), dict(bits=8), dict(order=None), dict(srt=None), dict(ws=None), dict(ws=P + 64), dict(order=P + 1)):
         assert sort(**bad) == einval, bad
     assert sort(size=size - 1) == ecap and sort(n=0, idx=None, order=None, srt=None, ws=None, size=0) == 0
-    size_b = l.lfs_embedding_bwd_workspace_bytes(5, 4)
-    def bwd(n=5, rows=3, width=4, v=P, t=0, order=P, srt=P, out=P, ws=P, size=size_b):
+    size_b = l.lfs_embedding_bwd_workspace_bytes(many, 4)
+    assert size_b > 0 and l.lfs_embedding_bwd_workspace_bytes(5, 4) == 0
+    def bwd(n=many, rows=3, width=4, v=P, t=0, order=P, srt=P, out=P, ws=P, size=size_b):
         return l.lfs_embedding_bwd(n, rows, width, v, t, order, srt, 1.0, 1, out, ws, size, None)
     for bad in (dict(n=-1), dict(rows=0), dict(width=0), dict(v=None), dict(t=5), dict(order=None), dict(srt=None), dict(out=None), dict(ws=None), dict(ws=P + 4), dict(out=P + 2),
-                dict(v=P + 1, t=2)):
+                dict(v=P + 1, t=2), dict(order=P + 4), dict(srt=P + 8)):
         assert bwd(**bad) == einval, bad
     assert bwd(size=size_b - 1) == ecap and bwd(n=0, v=None, order=None, srt=None, ws=None) == 0
 
