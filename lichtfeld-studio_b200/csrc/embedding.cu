@@ -398,6 +398,9 @@ SortWs carve_sort(int64_t n, const SortPlan& p, void* base) {
 //
 // Sums are held in two floats: a million gradients of one row lose nothing, and the result is the exact sum rounded once (but for ties), whatever the stretches. Sums in 64 bits
 // took 273 us for a million lookups of 45 columns where these took 84: 32-bit values become 64-bit ones at a small fraction of the rate that additions have.
+//
+// Bound by the latency of the rows, which lie anywhere in v_out: 1 M rows of 180 bytes take 248 MB from memory, 64 bytes at a time, 40 us at the copy rate; all of the gradient takes 61 us. Neither more
+// rows under way (eight, sixteen), nor more or fewer CTAs, nor copies to shared memory ahead (4 bytes a lane: 80 us) changed that.
 constexpr int kBwdThreads = 256, kTileUnits = 128;
 constexpr int64_t kOwnClear = 32768;   // elements of a table that a single CTA clears itself (a launch less: 1.5 us)
 // CTAs per SM by the sums that a lane holds
@@ -415,7 +418,12 @@ struct Sum {
         add(o.hi);
         lo = __fadd_rn(lo, o.lo);
     }
-    // the sum times scale, plus `more`, rounded once; once it is infinite or NaN the roundings say nothing
+    // the sum times scale, rounded once; once it is infinite or NaN the roundings say nothing
+    __device__ __forceinline__ float times(float scale) const {
+        const float p = __fmul_rn(hi, scale);
+        return isfinite(p) ? __fadd_rn(p, __fmaf_rn(lo, scale, __fmaf_rn(hi, scale, -p))) : p;
+    }
+    // and added to `more`
     __device__ __forceinline__ float times(float scale, float more) const {
         const float p = __fmul_rn(hi, scale);
         Sum r{more, __fmaf_rn(lo, scale, __fmaf_rn(hi, scale, -p))};
@@ -500,7 +508,7 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_ctas(C * V)) embedding_bwd_ke
             if (u < units) {
                 float* dst = v_table + (size_t)row * width + u * V;
 #pragma unroll
-                for (int j = 0; j < V; ++j) dst[j] = acc.get(k * V + j).times(scale, accumulate ? dst[j] : 0.0f);
+                for (int j = 0; j < V; ++j) dst[j] = accumulate ? acc.get(k * V + j).times(scale, dst[j]) : acc.get(k * V + j).times(scale);
             }
         }
     };
@@ -566,32 +574,53 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_ctas(C * V)) embedding_bwd_ke
         else write_row(row);
     }
     __syncthreads();
+    // Sums of the heads that follow one another: in the round of d, a group whose row has not ended in the d parts from its own on adds those of the next d.
+    bool stop = begin >= end || ends_s[g];
+    for (int d = 1; d < groups; d *= 2) {
+        const bool more = !stop && g + d < groups && (g + d) * share < total;
+        if (!__syncthreads_or(more)) break;
+        Sum sum[C * V];
+        bool then = true;
+        if (more) {
+            then = ends_s[g + d];
+#pragma unroll
+            for (int i = 0; i < C * V; ++i) {
+                sum[i] = head_s[i][threadIdx.x];
+                sum[i].add(head_s[i][threadIdx.x + (d << log_group)]);
+            }
+        }
+        __syncthreads();
+        if (more) {
+            stop = then;
+            if (lane == 0) ends_s[g] = then;
+#pragma unroll
+            for (int i = 0; i < C * V; ++i) head_s[i][threadIdx.x] = sum[i];
+        }
+        __syncthreads();
+    }
     // the row that goes on behind this group's part, and the one that the stretch begins inside of
-    auto join = [&](int32_t joined, bool from_head) {
-        int last = g + 1;
-        bool open = !from_head || !ends_s[0];
-        while (open && last * share < total) open = !ends_s[last++];   // parts g + 1 .. last - 1 begin inside the row
+    const bool opens = g == 0 && begin < end && from_before && first_row_s < rows;
+    const int next = g + 1;
+    const bool followed = next < groups && next * share < total;
 #pragma unroll
-        for (int k = 0; k < C; ++k) {
-            const int u = unit0 + (k << log_group);
+    for (int k = 0; k < C; ++k) {
+        const int u = unit0 + (k << log_group);
+        if (u >= units) continue;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                Sum sum = from_head ? head_s[k * V + j][threadIdx.x] : acc.get(k * V + j);
-                for (int h = g + 1; h < last; ++h) sum.add(head_s[k * V + j][(h << log_group) + lane]);
-                if (u < units) {
-                    const int col = u * V + j;
-                    if (from_head) parts[(size_t)(2 * (int64_t)blockIdx.x) * width + col] = sum;
-                    else if (open) parts[(size_t)(2 * (int64_t)blockIdx.x + 1) * width + col] = sum;
-                    else {
-                        float* dst = v_table + (size_t)joined * width + col;
-                        *dst = sum.times(scale, accumulate ? *dst : 0.0f);
-                    }
+        for (int j = 0; j < V; ++j) {
+            const int col = u * V + j;
+            if (opens) parts[(size_t)(2 * (int64_t)blockIdx.x) * width + col] = head_s[k * V + j][threadIdx.x];
+            if (tail) {
+                Sum sum = acc.get(k * V + j);
+                if (followed) sum.add(head_s[k * V + j][threadIdx.x + group]);
+                if (!followed || !ends_s[next]) parts[(size_t)(2 * (int64_t)blockIdx.x + 1) * width + col] = sum;
+                else {
+                    float* dst = v_table + (size_t)row * width + col;
+                    *dst = accumulate ? sum.times(scale, *dst) : sum.times(scale);
                 }
             }
         }
-    };
-    if (tail) join(row, false);
-    if (g == 0 && begin < end && from_before && first_row_s < rows) join(first_row_s, true);
+    }
 }
 
 // The rows that lie in several stretches: the one that has a row's tail adds the heads of those that follow. A CTA per stretch; its threads are columns by slices of the heads.
@@ -631,7 +660,7 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int64_t n,
         if (threadIdx.x < columns && col < width) {
             for (int k = 1; k < slices; ++k) acc.add(sum_s[threadIdx.x + k * columns]);
             float* dst = v_table + (size_t)row * width + col;
-            *dst = acc.times(scale, accumulate ? *dst : 0.0f);
+            *dst = accumulate ? acc.times(scale, *dst) : acc.times(scale);
         }
         __syncthreads();
     }
@@ -659,7 +688,7 @@ struct Bwd {
 };
 template <int DTYPE, int V, int C>
 int bwd(const Bwd& b) {
-    constexpr int T = C * V <= 4 ? 4 : C * V <= 8 ? 4 : 2;
+    constexpr int T = C * V <= 8 ? 4 : 2;
     const int column_tiles = (b.width / V + kTileUnits - 1) / kTileUnits;
     const Cut cut = bwd_cut(b.n, b.log_group, bwd_ctas(C * V), column_tiles);
     const bool alone = cut.stretches == 1 && column_tiles == 1 && b.rows * b.width <= kOwnClear;

@@ -52,7 +52,7 @@ struct AdamWArgs {
     AdamWTensor t[CAP];
     int32_t first[CAP + 1];   // tiles in front of tensor k
     int32_t n;
-    float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, bc2_sqrt_rcp, grad_scale;
+    float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, bc2_sqrt_rcp, grad_scale, minus_zero;
     uint32_t offset_m, offset_v;   // the step's part of the rounding thresholds
 };
 // under 4 KB and under 32 KB of arguments, which is what a launch takes
@@ -73,6 +73,13 @@ __device__ __forceinline__ void unpair(f32x2 v, float& a, float& b) { asm("mov.b
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) { f32x2 r; asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+// A product that is added to something and has to be rounded before that. A packed product and the sum behind it become one operation in spite of their .rn and of --fmad=false, and so
+// do a sum with a constant zero and what follows, so the zero (-0, which changes nothing) comes from the arguments.
+__device__ __forceinline__ f32x2 mul2_alone(f32x2 a, f32x2 b, f32x2 minus_zero) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(minus_zero));
+    return r;
+}
 
 // A lane's four elements.
 struct Block4 {
@@ -211,14 +218,15 @@ __device__ __forceinline__ float fast_root(float x) { float r; asm("sqrt.approx.
 __device__ __forceinline__ float fast_reciprocal(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
 struct Step {
-    float grad_scale, beta1, beta2, one_minus_beta1, one_minus_beta2, bc2_sqrt_rcp, eps, step_size, decay;
+    float grad_scale, beta1, beta2, one_minus_beta1, one_minus_beta2, bc2_sqrt_rcp, eps, minus_zero, step_size, decay;
 };
 __device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Block4& g, const Step& S) {
+    const f32x2 zero = pair(S.minus_zero, S.minus_zero);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const f32x2 gs = mul2(g.get(i), pair(S.grad_scale, S.grad_scale));
-        const f32x2 m1 = add2(mul2(m.get(i), pair(S.beta1, S.beta1)), mul2(gs, pair(S.one_minus_beta1, S.one_minus_beta1)));
-        const f32x2 v1 = add2(mul2(v.get(i), pair(S.beta2, S.beta2)), mul2(mul2(gs, pair(S.one_minus_beta2, S.one_minus_beta2)), gs));
+        const f32x2 m1 = add2(mul2_alone(m.get(i), pair(S.beta1, S.beta1), zero), mul2_alone(gs, pair(S.one_minus_beta1, S.one_minus_beta1), zero));
+        const f32x2 v1 = add2(mul2_alone(v.get(i), pair(S.beta2, S.beta2), zero), mul2_alone(mul2(gs, pair(S.one_minus_beta2, S.one_minus_beta2)), gs, zero));
         m.set(i, m1);
         v.set(i, v1);
         // The moments are rounded step by step, since their codes depend on it; the step itself takes the fast root and reciprocal, which are off by 2^-23 of it
@@ -271,6 +279,10 @@ __device__ __noinline__ void single_block(const AdamWTensor& T, uint32_t start, 
 // the tensor of tile q, which is not in front of tensor k's
 template <int CAP>
 __device__ __forceinline__ int tensor_of(const AdamWArgs<CAP>& A, int q, int k) {
+    if (CAP == kAdamWFew) {
+        while (q >= A.first[k + 1]) ++k;
+        return k;
+    }
     if (q < A.first[k + 1]) return k;
     int lo = k + 1, hi = A.n - 1;
     while (lo < hi) {
@@ -336,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
         stage = stage + 1 == kStages ? 0 : stage + 1;
         now = tensor_of(A, q, now);
         const AdamWTensor& T = A.t[now];
-        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, A.bc2_sqrt_rcp, A.eps, T.step_size, T.decay};
+        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, A.bc2_sqrt_rcp, A.eps, A.minus_zero, T.step_size, T.decay};
         const uint32_t tile = (uint32_t)(q - A.first[now]) * kTile;
         if (!(T.aligned && tile + kTile <= T.n)) {
             for (uint32_t start = tile + warp * kAdamWBlock; start < min(tile + kTile, T.n); start += kRow) single_block<8>(T, start, lane, S, A.offset_m, A.offset_v);
@@ -399,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, kCtas32) adamw32_kernel(const __grid
     for (int q = blockIdx.x; q < total; q += gridDim.x) {
         now = tensor_of(A, q, now);
         const AdamWTensor& T = A.t[now];
-        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, A.bc2_sqrt_rcp, A.eps, T.step_size, T.decay};
+        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, A.bc2_sqrt_rcp, A.eps, A.minus_zero, T.step_size, T.decay};
         const uint32_t tile = (uint32_t)(q - A.first[now]) * kRow, e = tile + t * 4;
         const bool whole = T.aligned && tile + kRow <= T.n;
         Block4 p{{p4.x, p4.y, p4.z, p4.w}}, m{{m4.x, m4.y, m4.z, m4.w}}, v{{v4.x, v4.y, v4.z, v4.w}}, g;
@@ -472,7 +484,7 @@ int launch_adamw(int count, const AdamWTensor* pieces, const Host& h) {
     }
     A.beta1 = (float)h.beta1; A.beta2 = (float)h.beta2;
     A.one_minus_beta1 = (float)(1.0 - h.beta1); A.one_minus_beta2 = (float)(1.0 - h.beta2);
-    A.eps = (float)h.eps; A.bc2_sqrt_rcp = (float)(1.0 / std::sqrt(1.0 - std::pow(h.beta2, (double)h.step_count))); A.grad_scale = h.grad_scale;
+    A.eps = (float)h.eps; A.bc2_sqrt_rcp = (float)(1.0 / std::sqrt(1.0 - std::pow(h.beta2, (double)h.step_count))); A.grad_scale = h.grad_scale; A.minus_zero = -0.0f;
     A.offset_m = (uint32_t)h.step_count * kGolden;
     A.offset_v = (uint32_t)h.step_count * kPlastic;
     LFS_TIMED("adamw", h.st);

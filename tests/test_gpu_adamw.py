@@ -434,3 +434,107 @@ def test_checkpoint_of_8_bit_moments_resumes_bit_for_bit(pkg, st, tmp_path):
         assert torch.equal(a._optimizer.exp_avg_sq.live(name)[0].view(torch.uint8), b._optimizer.exp_avg_sq.live(name)[0].view(torch.uint8))
     with pytest.raises(RuntimeError, match="moments in 8 bits"):
         fm.load_checkpoint(make(32), path)
+
+
+@pytest.mark.parametrize("grad", list(DTYPES))
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tiles_are_as_separate_tensors(st, bits, grad):
+    """A tensor of several tiles for every CTA of the GPU, next to small ones: the same bits as its pieces of 128 k elements each as a tensor of its own, but for the thresholds, which go by the
+    element's index in its tensor (so the comparison in 8 bits is of the parameters after the first step, which the rounding of the moments does not enter)."""
+    n = (1 << 17) * 30 + 77
+    P, G = tensor(n, seed=1), tensor(n, 0, DTYPES[grad], 0.1, seed=2)
+    Q = P.clone()
+    small = [tensor(100, seed=k) for k in range(3)]
+    one = st.AdamW([small[0], P, small[1]], [small[2], G, small[2]], lr=0.01, state_bits=bits)
+    one.step()
+    pieces = st.AdamW(list(Q.split(1 << 17)), list(G.split(1 << 17)), lr=0.01, state_bits=bits)
+    pieces.step()
+    assert torch.equal(P, Q)
+    if bits == 32:
+        one.step(), pieces.step()
+        assert torch.equal(P, Q) and torch.equal(one.moments[1].exp_avg_sq, torch.cat([m.exp_avg_sq for m in pieces.moments]))
+    else:
+        m = one.moments[1]
+        b1m, v = 0.1 * f64(G), 0.001 * f64(G) ** 2
+        check_codes(m.exp_avg, m.exp_avg_scale, b1m, 6 * U * np.abs(b1m) + 1e-44, 1, False)
+        check_codes(m.exp_avg_sq, m.exp_avg_sq_scale, v, 8 * U * v + 1e-44, 1, True)
+
+
+def test_two_optimizers_at_once(st):
+    """Steps of different tensors on two streams, and through two captured graphs, at the same time: nothing is shared."""
+    n = 300_000
+    def make(seed):
+        return st.AdamW([tensor(n, seed=seed)], [tensor(n, seed=seed + 1)], lr=0.01, state_bits=8)
+    a, b, c, d = make(1), make(5), make(1), make(5)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for opt, stream in ((a, streams[0]), (b, streams[1])):
+            with torch.cuda.stream(stream):
+                opt.step()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        c.step(), d.step()
+    for x, y in ((a, c), (b, d)):
+        assert torch.equal(x.params[0], y.params[0]) and torch.equal(x.moments[0].exp_avg.view(torch.uint8), y.moments[0].exp_avg.view(torch.uint8))
+
+
+def test_binding_and_refusals(st):
+    P, G = tensor(50), tensor(50, seed=1)
+    with pytest.raises(RuntimeError, match="overlap"):
+        st.AdamW([P, P[10:]], [G, G[10:]])
+    with pytest.raises(RuntimeError, match="elements"):
+        st.AdamW([P], [G[:40]])
+    with pytest.raises(RuntimeError, match="contiguous"):
+        st.AdamW([tensor(50).view(5, 10).t()], [G])
+    with pytest.raises(RuntimeError, match="grads"):
+        st.AdamW([P], [G.double()])
+    with pytest.raises(RuntimeError, match="for 1 tensors"):
+        st.AdamW([P], [G], lr=[0.1, 0.2])
+    with pytest.raises(RuntimeError, match="elements"):
+        st.AdamW([P], [G], moments=[st.Moments.zeros(40, 8, P.device)])
+    opt = st.AdamW([P], [None], lr=0.1)
+    before = P.clone()
+    opt.step()
+    assert torch.equal(P, before)
+    opt.set_grads([G])
+    opt.step()
+    assert not torch.equal(P, before) and opt.step_count == 2
+    # a rate changed by a scheduler counts from the next step on
+    opt.lr[0] = 0.0
+    before = P.clone()
+    opt.step()
+    assert torch.equal(P, before)
+    # the parameter's memory stays where the optimizer writes it
+    q = torch.nn.Parameter(tensor(30, seed=3))
+    opt = st.AdamW([q], [tensor(30, seed=4)])
+    q.data = torch.zeros(30, device="cuda")
+    opt.step()
+    torch.cuda.synchronize()
+    assert q.eq(0).all()
+
+
+@pytest.mark.parametrize("grad", list(DTYPES))
+def test_moments_are_rounded_operation_by_operation(st, pkg, grad):
+    """m = beta1 m + (1 - beta1) g and v = beta2 v + ((1 - beta2) g) g with every product and sum rounded to float32 (no fused ones), which decides the 8-bit codes: the same bits as torch's elementary
+    operations, in 32 bits and as scales and codes."""
+    n = 300_000
+    g = tensor(n, 0, DTYPES[grad], 0.1, seed=3)
+    p32, p8 = tensor(n, seed=1), tensor(n, seed=1)
+    a, b = st.AdamW([p32], [g], lr=0.01), st.AdamW([p8], [g], lr=0.01, state_bits=8)
+    m = v = torch.zeros(n, device="cuda")
+    m8, v8 = m.clone(), v.clone()
+    for t in range(1, 4):
+        gs = g.float() * 0.3
+        m, v = m * 0.9 + gs * (1 - 0.9), v * 0.999 + (gs * (1 - 0.999)) * gs
+        m8, v8 = m8 * 0.9 + gs * (1 - 0.9), v8 * 0.999 + (gs * (1 - 0.999)) * gs
+        a.step(0.3), b.step(0.3)
+        assert torch.equal(a.moments[0].exp_avg, m) and torch.equal(a.moments[0].exp_avg_sq, v)
+        held = b.moments[0]
+        for scale, x, top in ((held.exp_avg_scale, m8, 448.0), (held.exp_avg_sq_scale, v8, 57344.0)):
+            most = torch.nn.functional.pad(x.abs(), (0, -n % 128)).view(-1, 128).amax(1)
+            assert torch.equal(scale, most * torch.full_like(most, 1.0 / top))
+        # without an error of the value only the quotient and the product before the threshold's sum are rounded
+        check_codes(held.exp_avg, held.exp_avg_scale, f64(m8), np.zeros(n), t, False)
+        check_codes(held.exp_avg_sq, held.exp_avg_sq_scale, f64(v8), np.zeros(n), t, True)
+        m8, v8 = pkg.ops.adamw_state_decode(held.exp_avg, held.exp_avg_scale), pkg.ops.adamw_state_decode(held.exp_avg_sq, held.exp_avg_sq_scale)

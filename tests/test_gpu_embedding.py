@@ -194,6 +194,49 @@ def test_streams_and_graphs(ops):
         assert all(torch.equal(a, b) for a, b in zip(want, out))
 
 
+def test_long_gradient(ops):
+    """More lookups than a wave of CTAs takes in one round each: a row that spans many stretches next to short ones, rows without lookups, lookups that name no row at the end."""
+    n, rows = 1_200_003, 70_000
+    for width in (3, 16, 45):
+        gen = torch.Generator(device="cuda").manual_seed(width)
+        i = torch.randint(rows, (n,), device="cuda", generator=gen, dtype=torch.int32)
+        i[: n // 3] = 777
+        i[n // 3: n // 3 + 1000] = -1
+        v = torch.randn(n, width, device="cuda", generator=gen)
+        got = ops.embedding_bwd(v, ops.embedding_sort(i, rows), 1.0)
+        inside = i >= 0
+        want = torch.zeros(rows, width, device="cuda", dtype=torch.float64).index_add_(0, i[inside].long(), v[inside].double())
+        size = torch.zeros(rows, width, device="cuda", dtype=torch.float64).index_add_(0, i[inside].long(), v[inside].double().abs())
+        # two-float sums: U of the sum for its rounding, and n^2 U^2 < 0.006 U n of the magnitudes' mean is far below U / 1000 of their sum
+        assert ((got.double() - want).abs() <= U * want.abs() + U / 1000 * size + 1e-44).all()
+
+
+def test_infinite_gradients_stay_with_their_rows(ops):
+    v = randn(1000, 9, seed=2)
+    i = indices(1000, 20, kind="any")
+    v[100, 3], v[200, 4] = float("inf"), float("nan")
+    got = ops.embedding_bwd(v, ops.embedding_sort(i, 20), 0.5)
+    bad = torch.zeros(20, 9, dtype=torch.bool, device="cuda")
+    bad[i[100].long(), 3] = bad[i[200].long(), 4] = True
+    assert got[i[100].long(), 3].isinf() and got[i[200].long(), 4].isnan() and torch.isfinite(got[~bad]).all()
+
+
+def test_refusals(ops):
+    t, i = randn(6, 5), indices(10, 6)
+    for kw, message in ((dict(out=torch.empty(10, 4, device="cuda")), "hold 10 rows"), (dict(out=torch.empty(5, 10, device="cuda").t()), "contiguous"),
+                        (dict(out_dtype=torch.float16), "float32"), (dict(out=torch.empty(10, 5, device="cuda"), out_dtype=torch.float16), "out")):
+        with pytest.raises(RuntimeError, match=message):
+            ops.embedding_fwd(t, i, **kw)
+    order = ops.embedding_sort(i, 6)
+    for v, kw, message in ((randn(9, 5), {}, "v_out must be"), (randn(10, 5).double(), {}, "v_out must be"), (randn(5, 10).t(), {}, "contiguous"), (randn(10, 5), dict(accumulate=True), "out"),
+                           (randn(10, 5), dict(out=torch.empty(6, 4, device="cuda")), "6 rows"), (randn(10, 5), dict(out=torch.empty(6, 5, device="cuda").half()), "out must be")):
+        with pytest.raises(RuntimeError, match=message):
+            ops.embedding_bwd(v, order, **kw)
+    for rows in (0, -3, 1 << 31):
+        with pytest.raises(RuntimeError, match="bad sizes"):
+            ops.embedding_sort(i, rows)
+
+
 def test_palette_is_trained_with_the_scene(pkg, synth):
     """A palette of SH rows through render, loss and backward, its table and the scene's other groups updated by AdamW with 8-bit moments: the table's gradient is the
     sum of the shN gradients of each label, the run repeats bit for bit in what follows the render's atomic sums, and gradients agree with differences of the loss."""
