@@ -304,8 +304,9 @@ struct Stage {
 };
 static_assert(kThreads * 4 == kRow && kThreads * 16 == 2 * kTile, "one copy of 16 bytes a thread for both codes, and for 16-bit gradients");
 
-// Moments in 8 bits. Issue slots and memory are both near their limits, so the copies are wide and asynchronous: loads straight into registers wait for one another at every block, and cost
-// more instructions for their addresses.
+// Moments in 8 bits. Issue slots and memory are both near their limits (66 % and 63 % in a short run: 67 instructions for 16 bytes), so the copies are wide and asynchronous: loads straight into registers
+// wait for one another at every block and cost more instructions for their addresses. us for 3 M Gaussians at SH degree 3 (177 M elements): simple 1018, codes from scaled bits 755, the next block's loads under
+// way 592, tiles copied ahead 475 to 525. In a long run, where the clock is lower, 563 (79 % of the copy rate).
 template <int CAP>
 __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
     extern __shared__ __align__(128) char stages_s[];
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
     }
 }
 
-// Moments in 32 bits: nothing but memory. A tile is a block to a warp, and the next one's loads are under way while it is computed.
+// Moments in 32 bits: nothing but memory. A tile is a block to a warp, and the next one's loads are under way while it is computed: 59 M elements 258 us, 99 % of the copy rate (simple 321).
 template <int CAP>
 __global__ void __launch_bounds__(kThreads, kCtas32) adamw32_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x;
