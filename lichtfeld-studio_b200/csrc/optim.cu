@@ -151,27 +151,46 @@ __device__ __forceinline__ uint32_t encode4(const Block4& b, float inverse, uint
     }
     return codes;
 }
-// A block with numbers that are not finite: the others' scale is theirs alone.
 template <bool SECOND>
-__device__ __noinline__ uint32_t encode4_not_finite(Block4 b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
-    Block4 f;
+__device__ __forceinline__ uint32_t encode_block(const Block4& b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
+    // the scale of a block is that of its finite numbers alone
+    const bool finite = isfinite(warp_max(max4(b)));
+    Block4 f = b;
+    if (!finite)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) f.x[k] = isfinite(b.x[k]) ? b.x[k] : 0.0f;
+        for (int k = 0; k < 4; ++k) f.x[k] = isfinite(b.x[k]) ? b.x[k] : 0.0f;
     const Scaling s = scaling<SECOND>(warp_max(max4(f)));
     *scale = s.scale;
     uint32_t codes = encode4<SECOND>(f, s.inverse, e, offset, nearest);
+    if (!finite)
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (!isfinite(b.x[k])) codes = (codes & ~(0xFFu << (8 * k))) | (SECOND && isinf(b.x[k]) ? 0x7Cu : 0x7Fu) << (8 * k);
+        for (int k = 0; k < 4; ++k)
+            if (!isfinite(b.x[k])) codes = (codes & ~(0xFFu << (8 * k))) | (SECOND && isinf(b.x[k]) ? 0x7Cu : 0x7Fu) << (8 * k);
     return codes;
 }
-template <bool SECOND>
-__device__ __forceinline__ uint32_t encode_block(const Block4& b, uint32_t e, uint32_t offset, bool nearest, float* scale) {
-    const float most = warp_max(max4(b));
-    if (!isfinite(most)) return encode4_not_finite<SECOND>(b, e, offset, nearest, scale);
-    const Scaling s = scaling<SECOND>(most);
-    *scale = s.scale;
-    return encode4<SECOND>(b, s.inverse, e, offset, nearest);
+
+// Both moments of the warp's block. The scale is the first moment's in the lower half of the warp and the second's in the upper one, so that one division makes both.
+struct Codes { uint32_t m, v; float scale; };
+__device__ __noinline__ Codes encode_not_finite(Block4 m, Block4 v, uint32_t e, uint32_t offset_m, uint32_t offset_v) {
+    Codes c;
+    float ms, vs;
+    c.m = encode_block<false>(m, e, offset_m, false, &ms);
+    c.v = encode_block<true>(v, e, offset_v, false, &vs);
+    c.scale = threadIdx.x & 16 ? vs : ms;
+    return c;
+}
+__device__ __forceinline__ Codes encode_moments(const Block4& m, const Block4& v, uint32_t e, uint32_t offset_m, uint32_t offset_v) {
+    const float most_m = warp_max(max4(m)), most_v = warp_max(max4(v));
+    if (!isfinite(max_or_nan(most_m, most_v))) return encode_not_finite(m, v, e, offset_m, offset_v);
+    const bool upper = threadIdx.x & 16;
+    const float most = upper ? most_v : most_m;
+    const bool held = most >= kTiny;
+    const float inverse = held ? __fdiv_rn(upper ? kTopV : kTopM, most) : 0.0f;
+    Codes c;
+    c.m = encode4<false>(m, __shfl_sync(0xffffffffu, inverse, 0), e, offset_m, false);
+    c.v = encode4<true>(v, __shfl_sync(0xffffffffu, inverse, 16), e, offset_v, false);
+    c.scale = held ? __fmul_rn(most, upper ? 1.0f / kTopV : 1.0f / kTopM) : 0.0f;
+    return c;
 }
 
 // ---- memory ------------------------------------------------------------------------------------------
@@ -214,7 +233,8 @@ __device__ __forceinline__ void store4(uint8_t* dst, int64_t e, int64_t n, bool 
 __device__ __forceinline__ float half_bits(uint32_t bits, int dtype) {
     return dtype == LFS_BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
 }
-__device__ __forceinline__ float fast_root(float x) { float r; asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// of x, or of the smallest normal number where x is below it (2^-63, against an eps of 1e-8 or 1e-15): numbers under it take three more instructions
+__device__ __forceinline__ float fast_root(float x) { float r; asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(max_or_nan(x, 0x1p-126f))); return r; }
 __device__ __forceinline__ float fast_reciprocal(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
 struct Step {
@@ -230,7 +250,7 @@ __device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Bl
         m.set(i, m1);
         v.set(i, v1);
         // The moments are rounded step by step, since their codes depend on it; the step itself takes the fast root and reciprocal, which are off by 2^-23 of it
-        // (exact ones: two thirds more instructions). A denominator is zero or normal: the root of the smallest number is 2^-74.5.
+        // (exact ones: two thirds more instructions). A denominator is a normal number.
         float a, b;
         unpair(add2(mul2(pair(fast_root(v.x[2 * i]), fast_root(v.x[2 * i + 1])), pair(S.bc2_sqrt_rcp, S.bc2_sqrt_rcp)), pair(S.eps, S.eps)), a, b);
         const f32x2 step = mul2(mul2(m1, pair(S.step_size, S.step_size)), pair(fast_reciprocal(a), fast_reciprocal(b)));
@@ -262,14 +282,10 @@ __device__ __noinline__ void single_block(const AdamWTensor& T, uint32_t start, 
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (e + k >= n) m.x[k] = v.x[k] = 0.0f;
-        float ms, vs;
-        const uint32_t i = T.before + (uint32_t)e;
-        store4(static_cast<uint8_t*>(T.m), e, n, whole, encode_block<false>(m, i, offset_m, false, &ms));
-        store4(static_cast<uint8_t*>(T.v), e, n, whole, encode_block<true>(v, i, offset_v, false, &vs));
-        if (lane == 0) {
-            T.ms[start / kAdamWBlock] = ms;
-            T.vs[start / kAdamWBlock] = vs;
-        }
+        const Codes c = encode_moments(m, v, T.before + (uint32_t)e, offset_m, offset_v);
+        store4(static_cast<uint8_t*>(T.m), e, n, whole, c.m);
+        store4(static_cast<uint8_t*>(T.v), e, n, whole, c.v);
+        if ((lane & 15) == 0) (lane ? T.vs : T.ms)[start / kAdamWBlock] = c.scale;
     } else {
         store4(static_cast<float*>(T.m), e, n, whole, m);
         store4(static_cast<float*>(T.v), e, n, whole, v);
@@ -302,7 +318,7 @@ struct Stage {
     uint8_t m[kTile], v[kTile];
     float ms[kTile / kAdamWBlock], vs[kTile / kAdamWBlock];
 };
-static_assert(kThreads * 4 == kRow && kThreads * 16 == 2 * kTile, "one copy of 16 bytes a thread for both codes, and for 16-bit gradients");
+static_assert(kThreads * 4 == kRow && kTile % (8 * kThreads) == 0, "whole copies of 16 bytes a thread");
 
 // Moments in 8 bits. Issue slots and memory are both near their limits (66 % and 63 % in a short run: 67 instructions for 16 bytes), so the copies are wide and asynchronous: loads straight into registers
 // wait for one another at every block and cost more instructions for their addresses. us for 3 M Gaussians at SH degree 3 (177 M elements): simple 1018, codes from scaled bits 755, the next block's loads under
@@ -328,9 +344,16 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
                     const float* g = static_cast<const float*>(T.g) + start + t * 4;
 #pragma unroll
                     for (int k = 0; k < kBlocks; ++k) copy16(&s.g[k * kRow + t * 4], g + k * kRow);
-                } else copy16(&s.g[t * 4], static_cast<const uint16_t*>(T.g) + start + t * 8);
-                if (t < kTile / 16) copy16(&s.m[t * 16], static_cast<const uint8_t*>(T.m) + start + t * 16);
-                else copy16(&s.v[(t - kTile / 16) * 16], static_cast<const uint8_t*>(T.v) + start + (t - kTile / 16) * 16);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kTile / 8 / kThreads; ++k) copy16(&s.g[(k * kThreads + t) * 4], static_cast<const uint16_t*>(T.g) + start + (k * kThreads + t) * 8);
+                }
+#pragma unroll
+                for (int k = 0; k < kTile / 8 / kThreads; ++k) {
+                    const int piece = k * kThreads + t, of = piece % (kTile / 16) * 16;
+                    if (piece < kTile / 16) copy16(&s.m[of], static_cast<const uint8_t*>(T.m) + start + of);
+                    else copy16(&s.v[of], static_cast<const uint8_t*>(T.v) + start + of);
+                }
                 constexpr int kScales = kTile / kAdamWBlock / 4;
                 if (t < kScales) copy16(&s.ms[t * 4], T.ms + start / kAdamWBlock + t * 4);
                 else if (t < 2 * kScales) copy16(&s.vs[(t - kScales) * 4], T.vs + start / kAdamWBlock + (t - kScales) * 4);
@@ -359,6 +382,8 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
         const int dtype = T.grad_dtype;
         float* const p_out = T.p + e0;
         uint8_t *const m_out = static_cast<uint8_t*>(T.m) + e0, *const v_out = static_cast<uint8_t*>(T.v) + e0;
+        float* const scale_out = (lane & 16 ? T.vs : T.ms) + tile / kAdamWBlock + warp;
+        const uint32_t e_first = T.before + e0;
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
             const int i = k * kRow + t * 4;
@@ -372,14 +397,10 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
             v = decode_v(load4(s.v, i, 0, true), s.vs[k * kWarps + warp]);
             update(p, m, v, g, S);
             store4(p_out, k * kRow, 0, true, p);
-            float ms, vs;
-            const uint32_t e = T.before + e0 + k * kRow;
-            *reinterpret_cast<uint32_t*>(m_out + k * kRow) = encode_block<false>(m, e, A.offset_m, false, &ms);
-            *reinterpret_cast<uint32_t*>(v_out + k * kRow) = encode_block<true>(v, e, A.offset_v, false, &vs);
-            if (lane == 0) {
-                T.ms[tile / kAdamWBlock + k * kWarps + warp] = ms;
-                T.vs[tile / kAdamWBlock + k * kWarps + warp] = vs;
-            }
+            const Codes c = encode_moments(m, v, e_first + k * kRow, A.offset_m, A.offset_v);
+            *reinterpret_cast<uint32_t*>(m_out + k * kRow) = c.m;
+            *reinterpret_cast<uint32_t*>(v_out + k * kRow) = c.v;
+            if ((lane & 15) == 0) scale_out[k * kWarps] = c.scale;
         }
     }
 }
