@@ -53,7 +53,7 @@ Divide divide_by(uint32_t d) {
 //
 // Bound by the requests that an SM can send (76 % of their rate; a store is five, and 32 neighbouring elements lie in 2.7 lines of the table where rows are no whole number of lines): 1 M rows of 45
 // floats 43 us, 70 % of the copy rate, 3 M rows of 24 from half precision 53 us, 88 %. The same rows with a division for every element 79 us, with the rows' places in shared memory 48, copied to shared memory in 16-byte
-// pieces first 69, four neighbouring elements a thread 48.
+// pieces first 49 (by warps) to 69, four neighbouring elements a thread 48.
 constexpr int kFwdThreads = 128, kFwdUnroll = 8;
 template <int IN, int OUT, int V>
 __global__ void __launch_bounds__(kFwdThreads) embedding_fwd_kernel(int64_t n, int64_t rows, int units, Divide by_units, int segments, int segment,

@@ -233,8 +233,8 @@ __device__ __forceinline__ void store4(uint8_t* dst, int64_t e, int64_t n, bool 
 __device__ __forceinline__ float half_bits(uint32_t bits, int dtype) {
     return dtype == LFS_BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
 }
-// of x, or of the smallest normal number where x is below it (2^-63, against an eps of 1e-8 or 1e-15): numbers under it take three more instructions
-__device__ __forceinline__ float fast_root(float x) { float r; asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(max_or_nan(x, 0x1p-126f))); return r; }
+// (numbers below the normal ones included: beside an eps of 1e-15 the root of 2^-126 is 2e-4)
+__device__ __forceinline__ float fast_root(float x) { float r; asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float fast_reciprocal(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
 struct Step {
@@ -250,7 +250,7 @@ __device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Bl
         m.set(i, m1);
         v.set(i, v1);
         // The moments are rounded step by step, since their codes depend on it; the step itself takes the fast root and reciprocal, which are off by 2^-23 of it
-        // (exact ones: two thirds more instructions). A denominator is a normal number.
+        // (exact ones: two thirds more instructions). A denominator is zero or normal: the root of the smallest number is 2^-74.5.
         float a, b;
         unpair(add2(mul2(pair(fast_root(v.x[2 * i]), fast_root(v.x[2 * i + 1])), pair(S.bc2_sqrt_rcp, S.bc2_sqrt_rcp)), pair(S.eps, S.eps)), a, b);
         const f32x2 step = mul2(mul2(m1, pair(S.step_size, S.step_size)), pair(fast_reciprocal(a), fast_reciprocal(b)));
@@ -320,9 +320,9 @@ struct Stage {
 };
 static_assert(kThreads * 4 == kRow && kTile % (8 * kThreads) == 0, "whole copies of 16 bytes a thread");
 
-// Moments in 8 bits. Issue slots and memory are both near their limits (66 % and 63 % in a short run: 67 instructions for 16 bytes), so the copies are wide and asynchronous: loads straight into registers
-// wait for one another at every block and cost more instructions for their addresses. us for 3 M Gaussians at SH degree 3 (177 M elements): simple 1018, codes from scaled bits 755, the next block's loads under
-// way 592, tiles copied ahead 475 to 525. In a long run, where the clock is lower, 563 (79 % of the copy rate).
+// Moments in 8 bits. Issue slots and memory are both near their limits (62 instructions for 16 bytes), so the copies are wide and asynchronous: loads straight into registers wait for one another at every
+// block and cost more instructions for their addresses. us for 3 M Gaussians at SH degree 3 (177 M elements): simple 1018, codes from scaled bits 755, the next block's loads under way 592, tiles copied
+// ahead 515, one division and one check for both moments 450 (98 % of the copy rate). In a long run, where the clock is lower, 524 (84 %).
 template <int CAP>
 __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
     extern __shared__ __align__(128) char stages_s[];
@@ -510,9 +510,9 @@ int launch_adamw(int count, const AdamWTensor* pieces, const Host& h) {
     A.offset_m = (uint32_t)h.step_count * kGolden;
     A.offset_v = (uint32_t)h.step_count * kPlastic;
     LFS_TIMED("adamw", h.st);
-    // With 32 tiles to a CTA and more, three CTAs per SM: us for 0.5, 1, 2 and 3 M Gaussians at SH degree 3 with four 83, 165, 327 and 487, with three 84, 162, 319 and 475; 30 k and 120 k (degree 3) 9.7 and
-    // 26.8, 10.4 and 28.0. (Moments in 32 bits: 1 M in 295, 257 and 304 with four, three and two.)
-    if (BITS == 8) adamw8_kernel<CAP><<<grid_for(tiles, 1, tiles >= 32ll * kCtas8 * num_sms() ? kCtas8 - 1 : kCtas8), kThreads, kShared, h.st>>>(A);
+    // With 16 tiles to a CTA and more, three CTAs per SM: us for 0.25, 0.5, 1 and 3 M Gaussians at SH degree 3 with four 42.1, 82.7, 169 and 478, with three 42.2, 78.2, 151 and 450; 30 k and 120 k 9.6 and
+    // 25.5, 10.0 and 26.4. (Moments in 32 bits: 1 M in 295, 257 and 304 with four, three and two.)
+    if (BITS == 8) adamw8_kernel<CAP><<<grid_for(tiles, 1, tiles >= 16ll * kCtas8 * num_sms() ? kCtas8 - 1 : kCtas8), kThreads, kShared, h.st>>>(A);
     else adamw32_kernel<CAP><<<grid_for(tiles, 1, kCtas32), kThreads, 0, h.st>>>(A);
     return check_launch("adamw");
 }

@@ -538,3 +538,37 @@ def test_moments_are_rounded_operation_by_operation(st, pkg, grad):
         check_codes(held.exp_avg, held.exp_avg_scale, f64(m8), np.zeros(n), t, False)
         check_codes(held.exp_avg_sq, held.exp_avg_sq_scale, f64(v8), np.zeros(n), t, True)
         m8, v8 = pkg.ops.adamw_state_decode(held.exp_avg, held.exp_avg_scale), pkg.ops.adamw_state_decode(held.exp_avg_sq, held.exp_avg_sq_scale)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1e-15, 1e-8, 0.0])
+def test_steps_of_very_small_second_moments(st, pkg, bits, eps):
+    """Second moments of zero and below the smallest normal number next to first moments that are not zero, and very large gradients: the denominator is the formula's (2^-126 has the root 1.1e-19, which counts
+    beside an eps of 1e-15)."""
+    n = 512
+    v0 = torch.full((n,), 1e-40, device="cuda")
+    v0[:128] = 0.0
+    v0[256:384] = 1.2e-38
+    v0[384:] = 1e25
+    if bits == 8:
+        v0[128:256] = 1e-33        # just above 2^-110, below which 8 bits hold zeros
+    m0 = torch.linspace(0.5, 1.0, n, device="cuda") * 1e-16
+    m0[384:] = 1e11
+    g = torch.zeros(n, device="cuda")
+    P = torch.zeros(n, device="cuda")
+    if bits == 8:
+        codes = [pkg.ops.adamw_state_encode(m0), pkg.ops.adamw_state_encode(v0, True)]
+        m = st.Moments(codes[0][0], codes[1][0], codes[0][1], codes[1][1])
+        m0, v0 = (pkg.ops.adamw_state_decode(*c) for c in codes)
+    else:
+        m = st.Moments(m0.clone(), v0.clone())
+    opt = st.AdamW([P], [g], lr=1e-3, eps=eps, weight_decay=0.0, moments=[m])
+    opt.step_count = 99
+    opt.step()
+    m1, v1 = (m0 * 0.9).double(), (v0 * 0.999).double()
+    v1 = v1.float().double()                       # below the normal numbers a rounding is to a whole 2^-149
+    step = 1e-3 / (1 - B1 ** 100) * m1 / (torch.sqrt(v1 / (1 - B2 ** 100)) + eps)
+    got, want = P.double(), -step
+    held = torch.isfinite(want)
+    assert torch.equal(held, torch.isfinite(got)) and held[384:].all()
+    assert ((got - want).abs() <= 40 * U * want.abs())[held].all()
