@@ -320,9 +320,9 @@ struct Stage {
 };
 static_assert(kThreads * 4 == kRow && kTile % (8 * kThreads) == 0, "whole copies of 16 bytes a thread");
 
-// Moments in 8 bits. Issue slots and memory are both near their limits (62 instructions for 16 bytes), so the copies are wide and asynchronous: loads straight into registers wait for one another at every
+// Moments in 8 bits. Issue slots and memory are both near their limits (65 instructions for 16 bytes; 66 % of both), so the copies are wide and asynchronous: loads straight into registers wait for one another at every
 // block and cost more instructions for their addresses. us for 3 M Gaussians at SH degree 3 (177 M elements): simple 1018, codes from scaled bits 755, the next block's loads under way 592, tiles copied
-// ahead 515, one division and one check for both moments 450 (98 % of the copy rate). In a long run, where the clock is lower, 524 (84 %).
+// ahead 515, one division and one check for both moments 459 (96 % of the copy rate). In a long run, where the clock is lower, 503 (88 %).
 template <int CAP>
 __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
     extern __shared__ __align__(128) char stages_s[];
@@ -510,8 +510,8 @@ int launch_adamw(int count, const AdamWTensor* pieces, const Host& h) {
     A.offset_m = (uint32_t)h.step_count * kGolden;
     A.offset_v = (uint32_t)h.step_count * kPlastic;
     LFS_TIMED("adamw", h.st);
-    // With 16 tiles to a CTA and more, three CTAs per SM: us for 0.25, 0.5, 1 and 3 M Gaussians at SH degree 3 with four 42.1, 82.7, 169 and 478, with three 42.2, 78.2, 151 and 450; 30 k and 120 k 9.6 and
-    // 25.5, 10.0 and 26.4. (Moments in 32 bits: 1 M in 295, 257 and 304 with four, three and two.)
+    // With 16 tiles to a CTA and more, three CTAs per SM: us for 0.25, 0.5, 1 and 3 M Gaussians at SH degree 3 with four 42, 82, 168 and 478, with three 43, 79, 152 and 459; 30 k and 120 k 9.7 and 26.0,
+    // 10.1 and 27.0. (Moments in 32 bits: 1 M in 295, 257 and 304 with four, three and two.)
     if (BITS == 8) adamw8_kernel<CAP><<<grid_for(tiles, 1, tiles >= 16ll * kCtas8 * num_sms() ? kCtas8 - 1 : kCtas8), kThreads, kShared, h.st>>>(A);
     else adamw32_kernel<CAP><<<grid_for(tiles, 1, kCtas32), kThreads, 0, h.st>>>(A);
     return check_launch("adamw");
