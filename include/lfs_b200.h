@@ -470,8 +470,8 @@ int lfs_embedding_sort(int64_t n, int64_t rows, const void* indices, int index_b
 
 /* Gradient of lfs_embedding_fwd with respect to the table: v_table [rows,width] float32 = scale * sum over the lookups i of a row of
  * v_out[i] (v_out [n,width] of type `dtype`), zeros for rows without lookups; added to v_table with `accumulate`. order and sorted_rows are those of
- * lfs_embedding_sort for the same n and rows, 16-byte aligned. Sums are held in 32 bits and added in the order of the lookups' positions, in chunks
- * of fixed length: the result does not change from call to call. */
+ * lfs_embedding_sort for the same n and rows, 16-byte aligned. Sums are held in two floats each, so the result is the exact
+ * sum times scale, rounded once (but for ties), and does not change from call to call. */
 size_t lfs_embedding_bwd_workspace_bytes(int64_t n, int width);
 int lfs_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order,
                       const int32_t* sorted_rows, float scale, int accumulate, float* v_table, void* workspace,

@@ -169,6 +169,25 @@ def test_many_tensors_are_as_one_by_one(st, bits):
     assert all(torch.equal(a, b) for a, b in zip(before, after))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("count", [32, 33, 100, 128, 129, 424, 425])
+def test_each_length_of_list_is_as_one_by_one(st, bits, count):
+    """The lengths at which a launch takes other arguments: bit for bit what single steps give."""
+    sizes = [1 + (13 * i) % 331 + (4096 if i % 50 == 31 else 0) for i in range(count)]
+    def make():
+        return [tensor(n, 0, seed=i) for i, n in enumerate(sizes)], [tensor(n, 0, scale=0.1, seed=i + 5000) for i, n in enumerate(sizes)]
+    P, G = make()
+    opt = st.AdamW(P, G, lr=[1e-3 * (1 + i % 5) for i in range(count)], weight_decay=0.01, state_bits=bits)
+    opt.step(), opt.step()
+    Q, H = make()
+    for i in range(count):
+        one = st.AdamW([Q[i]], [H[i]], lr=1e-3 * (1 + i % 5), weight_decay=0.01, state_bits=bits)
+        one.step(), one.step()
+        assert torch.equal(P[i], Q[i])
+        for a, b in ((opt.moments[i].exp_avg, one.moments[0].exp_avg), (opt.moments[i].exp_avg_sq, one.moments[0].exp_avg_sq)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_gradients_that_are_not_finite_stay_with_their_elements(st):
     n = 1000
     for bits in (32, 8):
