@@ -403,8 +403,9 @@ SortWs carve_sort(int64_t n, const SortPlan& p, void* base) {
 // Sums are held in two floats: a million gradients of one row lose nothing, and the result is the exact sum rounded once (but for ties), whatever the stretches. Sums in 64 bits
 // took 273 us for a million lookups of 45 columns where these took 84: 32-bit values become 64-bit ones at a small fraction of the rate that additions have.
 //
-// Bound by the latency of the rows, which lie anywhere in v_out: 1 M rows of 180 bytes take 248 MB from memory, 64 bytes at a time, 40 us at the copy rate; all of the gradient takes 61 us. Neither more
-// rows under way (eight, sixteen), nor more or fewer CTAs, nor copies to shared memory ahead (4 bytes a lane: 80 us) changed that.
+// Bound by the loads of the rows, which lie anywhere in v_out: 1 M rows of 180 bytes take 248 MB from memory, 64 bytes at a time, 40 us at the copy rate; all of the gradient takes 61 us, 3 of them
+// the clearing and 5 embedding_join_kernel. Of the rest the sums are 2 and the looks for another row 4; rows that stay in L2 take 46. Neither more rows under way (eight, twelve, sixteen), nor the
+// next ones while these are added (62), nor more or fewer CTAs, nor a warp to a row of 45 columns (79), nor copies to shared memory ahead (4 bytes a lane: 80) changed that.
 constexpr int kBwdThreads = 256, kTileUnits = 128;
 constexpr int64_t kOwnClear = 32768;   // elements of a table that a single CTA clears itself (a launch less: 1.5 us)
 // CTAs per SM by the sums that a lane holds
