@@ -1018,7 +1018,8 @@ int lfs_adamw_step_tensors(int n_tensors, const lfs_adamw_tensor* tensors, doubl
     LFS_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || tensors), "bad tensor list");
     LFS_REQUIRE(step_count >= 1, "step_count must be >= 1");
     LFS_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "betas must be in [0, 1)");
-    LFS_REQUIRE(eps >= 0.0, "eps must not be negative");
+    // the reciprocal of the denominator takes numbers below the normal ones for zero, and its own largest are 2^126
+    LFS_REQUIRE(eps == 0.0 || (eps >= 0x1p-126 && eps <= 0x1p126), "eps must be zero or in [2^-126, 2^126]");
     for (int k = 0; k < n_tensors; ++k) {
         const lfs_adamw_tensor& t = tensors[k];
         LFS_REQUIRE(t.n >= 0 && t.n < (int64_t)1 << 37, "bad size");

@@ -250,7 +250,7 @@ __device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Bl
         m.set(i, m1);
         v.set(i, v1);
         // The moments are rounded step by step, since their codes depend on it; the step itself takes the fast root and reciprocal, which are off by 2^-23 of it
-        // (exact ones: two thirds more instructions). A denominator is zero or normal: the root of the smallest number is 2^-74.5.
+        // (exact ones: two thirds more instructions). A denominator is zero or normal: the root of the smallest number is 2^-74.5, and an eps below 2^-126 is refused.
         float a, b;
         unpair(add2(mul2(pair(fast_root(v.x[2 * i]), fast_root(v.x[2 * i + 1])), pair(S.bc2_sqrt_rcp, S.bc2_sqrt_rcp)), pair(S.eps, S.eps)), a, b);
         const f32x2 step = mul2(mul2(m1, pair(S.step_size, S.step_size)), pair(fast_reciprocal(a), fast_reciprocal(b)));

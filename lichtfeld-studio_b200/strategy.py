@@ -126,8 +126,8 @@ def _each(value, n: int, name: str) -> list:
 
 
 def _check_betas(betas, eps):
-    if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2 or not eps >= 0.0:
-        raise RuntimeError(f"betas must be two numbers in [0, 1) and eps not negative, got {betas}, {eps}")
+    if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2 or not (eps == 0.0 or 2.0 ** -126 <= eps <= 2.0 ** 126):
+        raise RuntimeError(f"betas must be two numbers in [0, 1) and eps zero or in [2^-126, 2^126], got {betas}, {eps}")
 
 
 class AdamW:
