@@ -419,7 +419,7 @@ int lfs_adam_step_segments(int n_segments, const lfs_adam_segment* segments /* h
 /* AdamW (Adam with decoupled weight decay) over any number of contiguous tensors, one launch per 424 of them (no counterpart
  * in the reference, whose optimizer has no weight decay and keeps 32-bit moments): what is trained next to the Gaussians (per-image
  * codes, exposure matrices, bilateral grids, palettes, small networks) and scenes whose moments should take a quarter of
- * the memory. With g = grad_scale * grad, t = step_count >= 1:
+ * the memory. With g = grad_scale * grad, t = step_count - missed >= 1, the number of this step for this tensor:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * Parameters are float32; gradients float32, bfloat16 or float16 (grad_dtype), computed with in 32 bits.
@@ -444,7 +444,7 @@ typedef struct lfs_adamw_tensor {
     float lr;
     float weight_decay;
     int32_t grad_dtype;        /* lfs_dtype */
-    int32_t reserved;
+    int32_t missed;            /* steps of the run that this tensor took no part in so far (0: none) */
 } lfs_adamw_tensor;
 int lfs_adamw_step_tensors(int n_tensors, const lfs_adamw_tensor* tensors /* host */, double beta1, double beta2, double eps,
                            int64_t step_count, float grad_scale, void* stream);

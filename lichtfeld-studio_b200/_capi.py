@@ -64,7 +64,7 @@ class AdamSegment(C.Structure):
 class AdamWTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
                 ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p), ("n", C.c_int64), ("lr", C.c_float),
-                ("weight_decay", C.c_float), ("grad_dtype", C.c_int32), ("reserved", C.c_int32)]
+                ("weight_decay", C.c_float), ("grad_dtype", C.c_int32), ("missed", C.c_int32)]
 
 
 class DpSegment(C.Structure):

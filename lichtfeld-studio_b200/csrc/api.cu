@@ -1024,6 +1024,7 @@ int lfs_adamw_step_tensors(int n_tensors, const lfs_adamw_tensor* tensors, doubl
         const lfs_adamw_tensor& t = tensors[k];
         LFS_REQUIRE(t.n >= 0 && t.n < (int64_t)1 << 37, "bad size");
         if (t.n == 0) continue;
+        LFS_REQUIRE(t.missed >= 0 && step_count - t.missed >= 1, "missed must be in [0, step_count)");
         LFS_REQUIRE(t.param && t.grad && t.exp_avg && t.exp_avg_sq, "null pointer in a tensor");
         LFS_REQUIRE(dtype_ok(t.grad_dtype), "grad_dtype must be LFS_F32, LFS_BF16 or LFS_F16");
         LFS_REQUIRE((t.exp_avg_scale == nullptr) == (t.exp_avg_sq_scale == nullptr), "both moments are held in 8 bits (two scale arrays) or both in 32 (none)");

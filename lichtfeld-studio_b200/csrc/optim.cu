@@ -9,7 +9,7 @@
 // How it is rounded decides whether 8 bits work at all. A second moment changes by 0.1 % a step and its codes are 12 to 25 % apart, so a value that
 // is rounded to the nearest code never leaves it (on gradients of changing visibility the moment settled at 1.5 times its mean, and what was rounded to zero took steps
 // thousands of times too long). Here element i of step t is rounded down, or up if its fraction of a code's distance plus a threshold reaches one:
-//   threshold_m = frac(i r1 + t r0), threshold_v = frac(i r0 + t r2), r0 the golden ratio's fraction, r1 and r2 those of the plastic number's powers
+//   threshold_m = frac(i r1 + t r0), threshold_v = frac(i r0 + t r2), t the tensor's own step number, r0 the golden ratio's fraction, r1 and r2 those of the plastic number's powers
 // The multiples of r0 and r2 spread evenly over [0, 1) (Weyl), so over the steps every moment moves by what it should on average, and a run can be
 // repeated bit for bit. The second moment is not rounded down to zero, which would leave the next denominator without its history. Same gradients, 6000 steps:
 // second moment 0.985 of its mean, path of the parameters 11 % off (the noise of the moments), against nearest codes 1.55 and thousands.
@@ -38,13 +38,19 @@ struct AdamWTensor {
     void *m, *v;          // float, or e4m3 and e5m2 codes
     float *ms, *vs;       // scales of the blocks; null with 32-bit moments
     uint32_t n;
-    uint32_t before;      // elements in front of these where a tensor is longer than kPiece, modulo 2^32
+    uint32_t flags;       // the gradient's type, kAligned, and in kBefore the elements in front of these where a tensor is longer than kPiece, modulo 2^32
     float step_size;      // lr / (1 - beta1^t)
     float decay;          // 1 - lr * weight decay
-    int32_t grad_dtype;
-    int32_t aligned;      // whole vectors can be read and written
+    float bc2_sqrt_rcp;   // 1 / sqrt(1 - beta2^t)
+    uint32_t t;           // this tensor's step number, modulo 2^32
+
+    __device__ __forceinline__ int grad_dtype() const { return (int)(flags & 3u); }
+    __device__ __forceinline__ bool aligned() const { return (flags & 4u) != 0; }
+    __device__ __forceinline__ uint32_t before() const { return flags & 0xC0000000u; }
 };
+constexpr uint32_t kAligned = 4;   // whole vectors can be read and written
 constexpr int64_t kPiece = (int64_t)1 << 30;
+static_assert(LFS_F32 < 4 && LFS_BF16 < 4 && LFS_F16 < 4, "");
 
 // A kernel takes its tensors as an argument: nothing is copied to the device or kept there, and a captured launch has its own copy.
 template <int CAP>
@@ -52,8 +58,7 @@ struct AdamWArgs {
     AdamWTensor t[CAP];
     int32_t first[CAP + 1];   // tiles in front of tensor k
     int32_t n;
-    float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, bc2_sqrt_rcp, grad_scale, minus_zero;
-    uint32_t offset_m, offset_v;   // the step's part of the rounding thresholds
+    float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, grad_scale, minus_zero;
 };
 // under 4, 10 and 32 KB of arguments, the most that a launch takes (a step of 40 small tensors 6.4 us with 10 KB and 8.1 with 32)
 constexpr int kAdamWFew = 32, kAdamWSome = 128, kAdamWMany = 424;
@@ -273,14 +278,14 @@ __device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Bl
 
 // A warp's block of a tile that is not whole, or of a tensor that cannot be read in vectors.
 template <int BITS>
-__device__ __noinline__ void single_block(const AdamWTensor& T, uint32_t start, int lane, const Step& S, uint32_t offset_m, uint32_t offset_v) {
+__device__ __noinline__ void single_block(const AdamWTensor& T, uint32_t start, int lane, const Step& S) {
     const int64_t e = (int64_t)start + lane * 4, n = T.n;
-    const bool whole = T.aligned && start + kAdamWBlock <= T.n;
+    const bool whole = T.aligned() && start + kAdamWBlock <= T.n;
     Block4 p = load4(T.p, e, n, whole), g, m, v;
-    if (T.grad_dtype == LFS_F32) g = load4(static_cast<const float*>(T.g), e, n, whole);
+    if (T.grad_dtype() == LFS_F32) g = load4(static_cast<const float*>(T.g), e, n, whole);
     else
 #pragma unroll
-        for (int k = 0; k < 4; ++k) g.x[k] = e + k < n ? half_bits(static_cast<const uint16_t*>(T.g)[e + k], T.grad_dtype) : 0.0f;
+        for (int k = 0; k < 4; ++k) g.x[k] = e + k < n ? half_bits(static_cast<const uint16_t*>(T.g)[e + k], T.grad_dtype()) : 0.0f;
     if constexpr (BITS == 8) {
         m = decode_m(load4(static_cast<const uint8_t*>(T.m), e, n, whole), T.ms[start / kAdamWBlock]);
         v = decode_v(load4(static_cast<const uint8_t*>(T.v), e, n, whole), T.vs[start / kAdamWBlock]);
@@ -295,7 +300,7 @@ __device__ __noinline__ void single_block(const AdamWTensor& T, uint32_t start, 
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (e + k >= n) m.x[k] = v.x[k] = 0.0f;
-        const Codes c = encode_moments(m, v, T.before + (uint32_t)e, offset_m, offset_v);
+        const Codes c = encode_moments(m, v, T.before() + (uint32_t)e, T.t * kGolden, T.t * kPlastic);
         store4(static_cast<uint8_t*>(T.m), e, n, whole, c.m);
         store4(static_cast<uint8_t*>(T.v), e, n, whole, c.v);
         if ((lane & 15) == 0) (lane ? T.vs : T.ms)[start / kAdamWBlock] = c.scale;
@@ -349,11 +354,11 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
             ahead = tensor_of(A, q, ahead);
             const AdamWTensor& T = A.t[ahead];
             const uint32_t start = (uint32_t)(q - A.first[ahead]) * kTile;
-            if (T.aligned && start + kTile <= T.n) {
+            if (T.aligned() && start + kTile <= T.n) {
                 const float* p = T.p + start + t * 4;
 #pragma unroll
                 for (int k = 0; k < kBlocks; ++k) copy16(&s.p[k * kRow + t * 4], p + k * kRow);
-                if (T.grad_dtype == LFS_F32) {
+                if (T.grad_dtype() == LFS_F32) {
                     const float* g = static_cast<const float*>(T.g) + start + t * 4;
 #pragma unroll
                     for (int k = 0; k < kBlocks; ++k) copy16(&s.g[k * kRow + t * 4], g + k * kRow);
@@ -385,18 +390,18 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
         stage = stage + 1 == kStages ? 0 : stage + 1;
         now = tensor_of(A, q, now);
         const AdamWTensor& T = A.t[now];
-        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, A.bc2_sqrt_rcp, A.eps, A.minus_zero, T.step_size, T.decay};
+        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, T.bc2_sqrt_rcp, A.eps, A.minus_zero, T.step_size, T.decay};
         const uint32_t tile = (uint32_t)(q - A.first[now]) * kTile;
-        if (!(T.aligned && tile + kTile <= T.n)) {
-            for (uint32_t start = tile + warp * kAdamWBlock; start < min(tile + kTile, T.n); start += kRow) single_block<8>(T, start, lane, S, A.offset_m, A.offset_v);
+        if (!(T.aligned() && tile + kTile <= T.n)) {
+            for (uint32_t start = tile + warp * kAdamWBlock; start < min(tile + kTile, T.n); start += kRow) single_block<8>(T, start, lane, S);
             continue;
         }
         const uint32_t e0 = tile + t * 4;
-        const int dtype = T.grad_dtype;
+        const int dtype = T.grad_dtype();
         float* const p_out = T.p + e0;
         uint8_t *const m_out = static_cast<uint8_t*>(T.m) + e0, *const v_out = static_cast<uint8_t*>(T.v) + e0;
         float* const scale_out = (lane & 16 ? T.vs : T.ms) + tile / kAdamWBlock + warp;
-        const uint32_t e_first = T.before + e0;
+        const uint32_t e_first = T.before() + e0, offset_m = T.t * kGolden, offset_v = T.t * kPlastic;
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
             const int i = k * kRow + t * 4;
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
             v = decode_v(load4(s.v, i, 0, true), s.vs[k * kWarps + warp]);
             update<true>(p, m, v, g, S);
             store4(p_out, k * kRow, 0, true, p);
-            const Codes c = encode_moments(m, v, e_first + k * kRow, A.offset_m, A.offset_v);
+            const Codes c = encode_moments(m, v, e_first + k * kRow, offset_m, offset_v);
             *reinterpret_cast<uint32_t*>(m_out + k * kRow) = c.m;
             *reinterpret_cast<uint32_t*>(v_out + k * kRow) = c.v;
             if ((lane & 15) == 0) scale_out[k * kWarps] = c.scale;
@@ -431,11 +436,11 @@ __global__ void __launch_bounds__(kThreads, kCtas32) adamw32_kernel(const __grid
         ahead = tensor_of(A, q, ahead);
         const AdamWTensor& T = A.t[ahead];
         const uint32_t tile = (uint32_t)(q - A.first[ahead]) * kRow, e = tile + t * 4;
-        if (!(T.aligned && tile + kRow <= T.n)) return;
+        if (!(T.aligned() && tile + kRow <= T.n)) return;
         p4 = *reinterpret_cast<const float4*>(T.p + e);
         m4 = *reinterpret_cast<const float4*>(static_cast<const float*>(T.m) + e);
         v4 = *reinterpret_cast<const float4*>(static_cast<const float*>(T.v) + e);
-        if (T.grad_dtype == LFS_F32) g4 = *reinterpret_cast<const uint4*>(static_cast<const float*>(T.g) + e);
+        if (T.grad_dtype() == LFS_F32) g4 = *reinterpret_cast<const uint4*>(static_cast<const float*>(T.g) + e);
         else {
             const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(T.g) + e);
             g4 = make_uint4(w.x, w.y, 0, 0);
@@ -446,19 +451,19 @@ __global__ void __launch_bounds__(kThreads, kCtas32) adamw32_kernel(const __grid
     for (int q = blockIdx.x; q < total; q += gridDim.x) {
         now = tensor_of(A, q, now);
         const AdamWTensor& T = A.t[now];
-        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, A.bc2_sqrt_rcp, A.eps, A.minus_zero, T.step_size, T.decay};
+        const Step S{A.grad_scale, A.beta1, A.beta2, A.one_minus_beta1, A.one_minus_beta2, T.bc2_sqrt_rcp, A.eps, A.minus_zero, T.step_size, T.decay};
         const uint32_t tile = (uint32_t)(q - A.first[now]) * kRow, e = tile + t * 4;
-        const bool whole = T.aligned && tile + kRow <= T.n;
+        const bool whole = T.aligned() && tile + kRow <= T.n;
         Block4 p{{p4.x, p4.y, p4.z, p4.w}}, m{{m4.x, m4.y, m4.z, m4.w}}, v{{v4.x, v4.y, v4.z, v4.w}}, g;
-        if (T.grad_dtype == LFS_F32) g = {__uint_as_float(g4.x), __uint_as_float(g4.y), __uint_as_float(g4.z), __uint_as_float(g4.w)};
-        else g = {half_bits(g4.x & 0xFFFFu, T.grad_dtype), half_bits(g4.x >> 16, T.grad_dtype), half_bits(g4.y & 0xFFFFu, T.grad_dtype), half_bits(g4.y >> 16, T.grad_dtype)};
+        if (T.grad_dtype() == LFS_F32) g = {__uint_as_float(g4.x), __uint_as_float(g4.y), __uint_as_float(g4.z), __uint_as_float(g4.w)};
+        else g = {half_bits(g4.x & 0xFFFFu, T.grad_dtype()), half_bits(g4.x >> 16, T.grad_dtype()), half_bits(g4.y & 0xFFFFu, T.grad_dtype()), half_bits(g4.y >> 16, T.grad_dtype())};
         load(q + gridDim.x);
         if (whole) {
             update<false>(p, m, v, g, S);
             store4(T.p, e, 0, true, p);
             store4(static_cast<float*>(T.m), e, 0, true, m);
             store4(static_cast<float*>(T.v), e, 0, true, v);
-        } else if (tile + warp * kAdamWBlock < T.n) single_block<32>(T, tile + warp * kAdamWBlock, lane, S, A.offset_m, A.offset_v);
+        } else if (tile + warp * kAdamWBlock < T.n) single_block<32>(T, tile + warp * kAdamWBlock, lane, S);
     }
 }
 
@@ -519,9 +524,7 @@ int launch_adamw(int count, const AdamWTensor* pieces, const Host& h) {
     }
     A.beta1 = (float)h.beta1; A.beta2 = (float)h.beta2;
     A.one_minus_beta1 = (float)(1.0 - h.beta1); A.one_minus_beta2 = (float)(1.0 - h.beta2);
-    A.eps = (float)h.eps; A.bc2_sqrt_rcp = (float)(1.0 / std::sqrt(1.0 - std::pow(h.beta2, (double)h.step_count))); A.grad_scale = h.grad_scale; A.minus_zero = -0.0f;
-    A.offset_m = (uint32_t)h.step_count * kGolden;
-    A.offset_v = (uint32_t)h.step_count * kPlastic;
+    A.eps = (float)h.eps; A.grad_scale = h.grad_scale; A.minus_zero = -0.0f;
     LFS_TIMED("adamw", h.st);
     // With 16 tiles to a CTA and more, three CTAs per SM: us for 0.25, 0.5, 1 and 3 M Gaussians at SH degree 3 with four 42, 82, 168 and 478, with three 43, 79, 152 and 459; 30 k and 120 k 9.7 and 26.0,
     // 10.1 and 27.0. (Moments in 32 bits: 1 M in 295, 257 and 304 with four, three and two.)
@@ -539,10 +542,16 @@ int launch_adamw_kind(int n_tensors, const lfs_adamw_tensor* tensors, const Host
         count = 0;
         return rc;
     };
-    const double bc1 = 1.0 / (1.0 - std::pow(h.beta1, (double)h.step_count));   // the same host arithmetic as lfs_adam_step_segments
+    int64_t step = 0;      // most tensors have the one number
+    double bc1 = 0.0, bc2_sqrt_rcp = 0.0;
     for (int k = 0; k < n_tensors; ++k) {
         const lfs_adamw_tensor& t = tensors[k];
         if ((t.exp_avg_scale != nullptr) != (BITS == 8)) continue;
+        if (t.n > 0 && h.step_count - t.missed != step) {
+            step = h.step_count - t.missed;
+            bc1 = 1.0 / (1.0 - std::pow(h.beta1, (double)step));   // the same host arithmetic as lfs_adam_step_segments
+            bc2_sqrt_rcp = 1.0 / std::sqrt(1.0 - std::pow(h.beta2, (double)step));
+        }
         const int grad_bytes = (int)dtype_bytes(t.grad_dtype), moment_bytes = BITS / 8;
         for (int64_t at = 0; at < t.n; at += kPiece) {
             if (count == kAdamWMany) {
@@ -557,11 +566,12 @@ int launch_adamw_kind(int n_tensors, const lfs_adamw_tensor* tensors, const Host
             o.ms = BITS == 8 ? t.exp_avg_scale + at / kAdamWBlock : nullptr;
             o.vs = BITS == 8 ? t.exp_avg_sq_scale + at / kAdamWBlock : nullptr;
             o.n = (uint32_t)std::min(t.n - at, kPiece);
-            o.before = (uint32_t)at;
             o.step_size = (float)((double)t.lr * bc1);
             o.decay = (float)(1.0 - (double)t.lr * (double)t.weight_decay);
-            o.grad_dtype = t.grad_dtype;
-            o.aligned = aligned_by(o.p, 16) && aligned_by(o.g, 16) && aligned_by(o.m, 16) && aligned_by(o.v, 16) && aligned_by(o.ms, 16) && aligned_by(o.vs, 16);
+            o.bc2_sqrt_rcp = (float)bc2_sqrt_rcp;
+            o.t = (uint32_t)step;
+            const bool aligned = aligned_by(o.p, 16) && aligned_by(o.g, 16) && aligned_by(o.m, 16) && aligned_by(o.v, 16) && aligned_by(o.ms, 16) && aligned_by(o.vs, 16);
+            o.flags = (uint32_t)t.grad_dtype | (aligned ? kAligned : 0u) | (uint32_t)at;
         }
     }
     return flush();

@@ -114,7 +114,7 @@ class Moments:
 
 
 _TABLE = np.dtype([("param", "u8"), ("grad", "u8"), ("exp_avg", "u8"), ("exp_avg_sq", "u8"), ("exp_avg_scale", "u8"), ("exp_avg_sq_scale", "u8"),
-                   ("n", "i8"), ("lr", "f4"), ("weight_decay", "f4"), ("grad_dtype", "i4"), ("reserved", "i4")])   # lfs_adamw_tensor
+                   ("n", "i8"), ("lr", "f4"), ("weight_decay", "f4"), ("grad_dtype", "i4"), ("missed", "i4")])   # lfs_adamw_tensor
 
 
 def _each(value, n: int, name: str) -> list:
@@ -135,8 +135,9 @@ class AdamW:
     palettes, small networks. Parameters are contiguous float32, gradients contiguous float32, bfloat16 or float16 of the same number of elements, on one device.
 
     Parameters, gradients and moments are bound here and stay bound: a step reads the gradients that are in those buffers by then (torch: zero_grad(set_to_none=False)),
-    and set_grads binds others. None in the place of a gradient leaves its parameter out. `lr` and `weight_decay` (one value or one per tensor) are
-    read at every step, so a scheduler may change them. moments: those of a run to continue; else zeros, in state_bits (32 or 8) bits."""
+    and set_grads binds others. None in the place of a gradient leaves its parameter out, and the step does not count for it: `missed` [tensors] is how many of the step_count steps so far each one took no
+    part in, and step_count - missed is the number that its bias corrections go by. `lr` and `weight_decay` (one value or one per tensor) are
+    read at every step, so a scheduler may change them. moments: those of a run to continue, with its step_count and missed to be set as well; else zeros, in state_bits (32 or 8) bits."""
 
     def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, moments=None):
         params = list(params)
@@ -162,6 +163,7 @@ class AdamW:
         self.lr, self.weight_decay = _each(lr, n, "lr"), _each(weight_decay, n, "weight_decay")
         self.step_count = 0
         self._table, self._rates = np.zeros(n, _TABLE), None
+        self.missed = self._table["missed"]
         self._address = self._table.ctypes.data
         self._table["param"] = [p.data_ptr() for p in self.params]
         for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
@@ -186,6 +188,8 @@ class AdamW:
             if g.numel() != p.numel():
                 raise RuntimeError(f"grads[{i}] must have {p.numel()} elements, got {g.numel()}")
         self.grads = [None if g is None else g.detach() for g in grads]
+        absent = np.array([g is None for g in grads])
+        self._absent = absent if absent.any() else None
         self._table["n"] = [0 if g is None else g.numel() for g in grads]
         self._table["grad"] = [0 if g is None else g.data_ptr() for g in grads]
         self._table["grad_dtype"] = [0 if g is None else ops._DTYPES[g.dtype] for g in grads]
@@ -199,6 +203,8 @@ class AdamW:
         ops._call_on(self.device, "lfs_adamw_step_tensors", len(self._table), self._address, self.betas[0], self.betas[1], self.eps,
                      self.step_count + 1, float(grad_scale))
         self.step_count += 1
+        if self._absent is not None:
+            self.missed[self._absent] += 1
 
 
 class PackedMoments:

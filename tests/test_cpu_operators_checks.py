@@ -32,3 +32,9 @@ def test_eps_of_zero_and_of_the_smallest_normal_number_are_served(pkg):
     for eps in (0.0, 2.0 ** -126, 1e-15, 1.0):
         assert pkg.strategy.FusedAdamW(model, [1e-3] * 6, eps=eps).eps == eps
         assert adamw(pkg, eps=eps, n=0) == 0
+
+
+def test_a_step_number_below_one_is_refused(pkg):
+    for step, missed in ((5, 5), (5, 9), (5, -1), (1, 1)):
+        assert adamw(pkg, step=step, missed=missed) == pkg._capi.LFS_EINVAL and "missed" in pkg._capi.lib().lfs_last_error().decode()
+    assert adamw(pkg, step=5, missed=9, n=0) == 0     # a tensor that takes no part
