@@ -12,6 +12,7 @@ step() explicitly because there is no autograd .grad slot."""
 from __future__ import annotations
 
 import ctypes as C
+import numbers
 from dataclasses import dataclass
 
 import numpy as np
@@ -119,7 +120,7 @@ _TABLE = np.dtype([("param", "u8"), ("grad", "u8"), ("exp_avg", "u8"), ("exp_avg
 
 def _each(value, n: int, name: str) -> list:
     """One float per tensor from one for all or a list."""
-    values = [float(value)] * n if isinstance(value, (int, float)) else [float(x) for x in value]
+    values = [float(value)] * n if isinstance(value, numbers.Real) else [float(x) for x in value]
     if len(values) != n:
         raise RuntimeError(f"{name}: {len(values)} values for {n} tensors")
     return values
@@ -137,7 +138,7 @@ class AdamW:
     Parameters, gradients and moments are bound here and stay bound: a step reads the gradients that are in those buffers by then (torch: zero_grad(set_to_none=False)),
     and set_grads binds others. None in the place of a gradient leaves its parameter out, and the step does not count for it: `missed` [tensors] is how many of the step_count steps so far each one took no
     part in, and step_count - missed is the number that its bias corrections go by. `lr` and `weight_decay` (one value or one per tensor) are
-    read at every step, so a scheduler may change them. moments: those of a run to continue, with its step_count and missed to be set as well; else zeros, in state_bits (32 or 8) bits."""
+    read at every step, so a scheduler may change one entry or set the whole again (one value or one per tensor). moments: those of a run to continue, with its step_count and missed to be set as well; else zeros, in state_bits (32 or 8) bits."""
 
     def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, moments=None):
         params = list(params)
@@ -160,7 +161,7 @@ class AdamW:
             raise RuntimeError(f"moments: {len(self.moments)} for {n} tensors")
         for i, (p, m) in enumerate(zip(self.params, self.moments)):
             m.check(p.numel(), self.device, f"moments[{i}]")
-        self.lr, self.weight_decay = _each(lr, n, "lr"), _each(weight_decay, n, "weight_decay")
+        self.lr, self.weight_decay = lr, weight_decay
         self.step_count = 0
         self._table, self._rates = np.zeros(n, _TABLE), None
         self.missed = self._table["missed"]
@@ -169,6 +170,22 @@ class AdamW:
         for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
             self._table[name] = [0 if getattr(m, name) is None else getattr(m, name).data_ptr() for m in self.moments]
         self.set_grads(grads)
+
+    @property
+    def lr(self) -> list:
+        return self._lr
+
+    @lr.setter
+    def lr(self, value):
+        self._lr = _each(value, len(self.params), "lr")
+
+    @property
+    def weight_decay(self) -> list:
+        return self._weight_decay
+
+    @weight_decay.setter
+    def weight_decay(self, value):
+        self._weight_decay = _each(value, len(self.params), "weight_decay")
 
     @staticmethod
     def _bits(state_bits, n):
@@ -196,9 +213,10 @@ class AdamW:
 
     def step(self, grad_scale: float = 1.0):
         """One update from the bound gradients, which grad_scale multiplies."""
-        rates = (list(self.lr), list(self.weight_decay))
+        rates = (list(self._lr), list(self._weight_decay))
         if rates != self._rates:
-            self._table["lr"], self._table["weight_decay"] = rates
+            for name, values in zip(("lr", "weight_decay"), rates):
+                self._table[name] = _each(values, len(self.params), name)
             self._rates = rates
         ops._call_on(self.device, "lfs_adamw_step_tensors", len(self._table), self._address, self.betas[0], self.betas[1], self.eps,
                      self.step_count + 1, float(grad_scale))
