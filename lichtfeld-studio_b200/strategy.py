@@ -150,9 +150,6 @@ class AdamW:
         self.device = params[0].device
         for i, p in enumerate(params):
             ops._check_typed(p, f"params[{i}]", (torch.float32,), self.device)
-        spans = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in params if p.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise RuntimeError("params must not overlap")
         self.params = [p.detach() for p in params]   # keeps the memory that the kernel writes to
         if moments is None:
             moments = [Moments.zeros(p.numel(), b, self.device) for p, b in zip(self.params, self._bits(state_bits, n))]
@@ -169,6 +166,7 @@ class AdamW:
         self._table["param"] = [p.data_ptr() for p in self.params]
         for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
             self._table[name] = [0 if getattr(m, name) is None else getattr(m, name).data_ptr() for m in self.moments]
+        self._check_written([p.numel() for p in self.params])
         self.set_grads(grads)
 
     @property
@@ -193,6 +191,18 @@ class AdamW:
         if len(bits) != n:
             raise RuntimeError(f"state_bits: {len(bits)} values for {n} tensors")
         return bits
+
+    def _check_written(self, sizes):
+        """A step writes parameters, moments and scales in one launch, in no order."""
+        t, n = self._table, np.array(sizes, dtype=np.int64)
+        one = np.where(t["exp_avg_scale"] == 0, 4, 1)
+        starts = np.concatenate([t[x].astype(np.int64) for x in ("param", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")])
+        scales = np.where(t["exp_avg_scale"] == 0, 0, -(-n // capi.LFS_ADAMW_BLOCK) * 4)
+        ends = starts + np.concatenate([4 * n, one * n, one * n, scales, scales])
+        some = ends > starts
+        order = np.argsort(starts[some])
+        if (ends[some][order][:-1] > starts[some][order][1:]).any():
+            raise RuntimeError("params and moments must not overlap")
 
     def set_grads(self, grads):
         grads = list(grads)
