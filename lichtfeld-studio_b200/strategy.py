@@ -297,6 +297,8 @@ class FusedAdamW(FusedAdam):
     def step(self, iteration: int, grads: SplatData, grad_scale: float = 1.0, first_row: int = 0, n_rows=None, rasterizer=None):
         if rasterizer is not None or first_row != 0 or n_rows not in (None, self.model.size):
             raise RuntimeError("FusedAdamW updates all rows from materialised gradients")
+        if grads.K != self.model.K or grads.capacity < self.model.size or grads.flat.device != self.model.flat.device:
+            raise RuntimeError(f"gradients of {grads.capacity} rows with {grads.K} SH bases on {grads.flat.device} for {self.model.size} with {self.model.K} on {self.model.flat.device}")
         self.exp_avg.size = self.exp_avg_sq.size = grads.size = self.model.size
         packed = self.state_bits == 8
         for i, name in enumerate(PARAM_NAMES):

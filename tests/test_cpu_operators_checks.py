@@ -38,3 +38,15 @@ def test_a_step_number_below_one_is_refused(pkg):
     for step, missed in ((5, 5), (5, 9), (5, -1), (1, 1)):
         assert adamw(pkg, step=step, missed=missed) == pkg._capi.LFS_EINVAL and "missed" in pkg._capi.lib().lfs_last_error().decode()
     assert adamw(pkg, step=5, missed=9, n=0) == 0     # a tensor that takes no part
+
+
+def test_gradients_of_another_scene_are_refused(pkg):
+    """FusedAdamW reads as many gradient rows as the model has."""
+    st, tr = pkg.strategy, pkg.trainer
+    cpu = torch.device("cpu")
+    opt = st.FusedAdamW(tr.SplatData(10, 4, cpu), [1e-3] * 6, state_bits=8)
+    for grads in (tr.SplatData(4, 4, cpu), tr.SplatData(10, 9, cpu), tr.SplatData(10, 4, torch.device("meta"))):
+        size = grads.size
+        with pytest.raises(RuntimeError, match="gradients"):
+            opt.step(2000, grads)
+        assert grads.size == size and opt.step_count == 0
