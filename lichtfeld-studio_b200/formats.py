@@ -6,7 +6,7 @@
   logit opacity / log scale, normalised quaternions. The interleaved rows are built on the device by one kernel
   (`lfs_ply_pack_rows`) and cross PCIe once through a pinned buffer.
 * Checkpoint (no counterpart file format in the reference, which resumes from PLY only): parameters, both Adam
-  moments, the step count, learning rates and strategy counters in one flat binary file:
+  moments, the optimizer and its step count, learning rates, weight decays and strategy counters in one flat binary file:
       magic "LFSCKPT1" | uint64 header length | JSON header | float32 payload (params, exp_avg, exp_avg_sq rows)
   Each payload section is the six groups [means | sh0 | shN | scaling | rotation | opacity] of the LIVE rows; 8-bit moments
   (header "state_bits": 8) are stored as they are held, the codes of a group and then its float32 scales."""
@@ -22,7 +22,7 @@ import torch
 
 from . import _capi as capi
 from ._capi import call, ptr
-from .strategy import PackedMoments
+from .strategy import FusedAdamW, PackedMoments
 from .trainer import PARAM_NAMES, SplatData
 
 _MAGIC = b"LFSCKPT1"
@@ -132,6 +132,10 @@ def _sections(strategy):
     return [("params", strategy.get_model()), ("exp_avg", opt.exp_avg), ("exp_avg_sq", opt.exp_avg_sq)]
 
 
+def _optimizer_kind(opt) -> str:
+    return "adamw" if isinstance(opt, FusedAdamW) else "adam"
+
+
 def _live_buffers(sd, name):
     """The tensors that hold one group's live rows, with the numpy type they are written as."""
     if isinstance(sd, PackedMoments):
@@ -142,12 +146,14 @@ def _live_buffers(sd, name):
 
 def save_checkpoint(strategy, path: str, iteration: int) -> str:
     """Everything needed to continue training bit-identically: live rows of the parameters and both Adam moments,
-    optimizer step count, per-group learning rates (after decay), active SH degree and the iteration."""
+    optimizer kind and step count, per-group learning rates (after decay) and weight decays, active SH degree and the iteration."""
     model, opt = strategy.get_model(), strategy._optimizer
     n = model.size
     header = dict(version=1, iteration=int(iteration), n=n, sh_coeffs=model.K, step_count=int(opt.step_count), lr=list(opt.lr),
                   betas=list(opt.betas), eps=opt.eps, active_sh_degree=int(getattr(strategy, "active_sh_degree", 0)),
-                  strategy=type(strategy).__name__, state_bits=getattr(opt, "state_bits", 32), sections=[s for s, _ in _sections(strategy)], groups=list(PARAM_NAMES))
+                  strategy=type(strategy).__name__, optimizer=_optimizer_kind(opt), state_bits=getattr(opt, "state_bits", 32), sections=[s for s, _ in _sections(strategy)], groups=list(PARAM_NAMES))
+    if isinstance(opt, FusedAdamW):
+        header["weight_decay"] = list(opt.weight_decay)
     hj = json.dumps(header).encode("utf-8")
     tmp = path + ".tmp"
     with open(tmp, "wb") as f:
@@ -178,6 +184,8 @@ def load_checkpoint(strategy, path: str) -> int:
             raise RuntimeError(f"{path}: {n} Gaussians exceed the model's capacity {model.capacity}")
         if header.get("groups") != list(PARAM_NAMES):
             raise RuntimeError(f"{path}: unexpected group order")
+        if header.get("optimizer", _optimizer_kind(opt)) != _optimizer_kind(opt):   # older files do not say
+            raise RuntimeError(f"{path}: made with optimizer={header['optimizer']!r}, the strategy has {_optimizer_kind(opt)!r}")
         if header.get("state_bits", 32) != getattr(opt, "state_bits", 32):
             raise RuntimeError(f"{path}: moments in {header.get('state_bits', 32)} bits, the optimizer keeps {getattr(opt, 'state_bits', 32)}")
         for _, sd in _sections(strategy):
@@ -193,6 +201,8 @@ def load_checkpoint(strategy, path: str) -> int:
         strategy.grads.size = n
     opt.step_count = int(header["step_count"])
     opt.lr = [float(x) for x in header["lr"]]
+    if "weight_decay" in header:
+        opt.weight_decay = [float(x) for x in header["weight_decay"]]
     if hasattr(strategy, "active_sh_degree"):
         strategy.active_sh_degree = int(header["active_sh_degree"])
     return int(header["iteration"])

@@ -50,3 +50,66 @@ def test_gradients_of_another_scene_are_refused(pkg):
         with pytest.raises(RuntimeError, match="gradients"):
             opt.step(2000, grads)
         assert grads.size == size and opt.step_count == 0
+
+
+# ---- checkpoints ----------------------------------------------------------------------------------------------------
+def strategy(pkg, kind="MCMC", **kw):
+    st, tr = pkg.strategy, pkg.trainer
+    model = tr.SplatData(9, 4, "cpu", capacity=16)
+    params = dict(max_cap=16, sh_degree=1)
+    params.update(kw)
+    s = getattr(st, kind)(model)
+    s.initialize(st.DefaultStrategy.Parameters(**params) if kind == "DefaultStrategy" else st.OptimizationParameters(**params))
+    return s
+
+
+@pytest.mark.parametrize("kind", ["MCMC", "DefaultStrategy"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_checkpoint_keeps_the_weight_decay(pkg, tmp_path, kind, bits):
+    a = strategy(pkg, kind, optimizer="adamw", weight_decay=(0.0, 0.1, 0.2, 0.0, 0.3, 0.0), state_bits=bits)
+    a._optimizer.weight_decay[5] = 0.7      # changed during the run, like a learning rate
+    path = pkg.formats.save_checkpoint(a, str(tmp_path / "a.ckpt"), 100)
+    b = strategy(pkg, kind, optimizer="adamw", weight_decay=0.05, state_bits=bits)
+    assert pkg.formats.load_checkpoint(b, path) == 100
+    assert b._optimizer.weight_decay == [0.0, 0.1, 0.2, 0.0, 0.3, 0.7]
+
+
+def test_a_checkpoint_of_another_optimizer_is_refused(pkg, tmp_path):
+    fm = pkg.formats
+    path = fm.save_checkpoint(strategy(pkg, optimizer="adamw", weight_decay=0.1), str(tmp_path / "a.ckpt"), 1)
+    with pytest.raises(RuntimeError, match="optimizer"):
+        fm.load_checkpoint(strategy(pkg), path)
+    path = fm.save_checkpoint(strategy(pkg), str(tmp_path / "b.ckpt"), 1)
+    with pytest.raises(RuntimeError, match="optimizer"):
+        fm.load_checkpoint(strategy(pkg, optimizer="adamw"), path)
+
+
+def test_a_refused_checkpoint_changes_nothing(pkg, tmp_path):
+    fm = pkg.formats
+    path = fm.save_checkpoint(strategy(pkg, optimizer="adamw"), str(tmp_path / "a.ckpt"), 1)
+    b = strategy(pkg)
+    b.get_model().size = 5
+    before = b.get_model().flat.clone()
+    with pytest.raises(RuntimeError):
+        fm.load_checkpoint(b, path)
+    assert b.get_model().size == 5 and torch.equal(b.get_model().flat, before)
+
+
+def test_a_checkpoint_without_these_fields_is_still_read(pkg, tmp_path):
+    """As written before they were there: plain Adam's, and AdamW's with the caller's weight decay."""
+    import json
+    import struct
+    fm = pkg.formats
+    for kw in ({}, dict(optimizer="adamw", weight_decay=0.25)):
+        path = fm.save_checkpoint(strategy(pkg, **kw), str(tmp_path / "a.ckpt"), 7)
+        raw = open(path, "rb").read()
+        (length,) = struct.unpack("<Q", raw[8:16])
+        header = json.loads(raw[16:16 + length])
+        header.pop("optimizer", None), header.pop("weight_decay", None)
+        head = json.dumps(header).encode()
+        with open(path, "wb") as f:
+            f.write(raw[:8] + struct.pack("<Q", len(head)) + head + raw[16 + length:])
+        b = strategy(pkg, **kw)
+        assert fm.load_checkpoint(b, path) == 7
+        if kw:
+            assert b._optimizer.weight_decay == [0.25] * 6
