@@ -440,12 +440,8 @@ class MCMC(IStrategy):
         new_n = int(keep.numel())
         if new_n == old_n:
             return
-        for sd in (self._splat_data, self._optimizer.exp_avg, self._optimizer.exp_avg_sq):
-            sd.size = old_n  # every buffer is gathered with indices into the OLD row range
-            kept = {n: sd.tensor(n).index_select(0, keep) for n in ("means", "sh0", "shN", "scaling_raw", "rotation_raw", "opacity_raw")}
-            sd.size = new_n
-            for n, t in kept.items():
-                sd.put(n, t)
+        _rewrite_rows((self._splat_data, self._optimizer.exp_avg, self._optimizer.exp_avg_sq), old_n, new_n,
+                      lambda _, name, rows: rows.index_select(0, keep))
         self.grads.size = new_n
         self._grads_valid = False
 
@@ -525,16 +521,20 @@ class MCMC(IStrategy):
              ptr(noise), ptr(sd._full["means"]), current_lr, _stream())
 
 
-def _rewrite_rows(buffers, new_rows: dict, new_n: int):
-    """Replace the live rows of several SplatData buffers (parameters, moments) by freshly gathered rows.
-    new_rows[i] is a dict name -> tensor for buffers[i]; counterpart of update_param_with_optimizer
-    (src/training/strategies/strategy_utils.cpp:57) on capacity-reserved storage."""
-    for sd, rows in zip(buffers, new_rows):
+def _rewrite_rows(buffers, old_n: int, new_n: int, new_rows):
+    """Replace the live rows of several buffers (parameters, moments) by new_rows(index of the buffer, group, its old rows), one
+    group at a time: besides the buffers there are never more than the old and the new rows of one group (moments in 8 bits are
+    decoded for this). Counterpart of update_param_with_optimizer (src/training/strategies/strategy_utils.cpp:57) on
+    capacity-reserved storage. new_rows reads nothing but the rows that it is given."""
+    for sd in buffers:
         if new_n > sd.capacity:
             raise RuntimeError("SplatData capacity exhausted: reserve more rows")
-        sd.size = new_n
-        for name, t in rows.items():
-            sd.put(name, t)
+    for i, sd in enumerate(buffers):
+        for name in PARAM_NAMES:
+            sd.size = old_n
+            rows = new_rows(i, name, sd.tensor(name))
+            sd.size = new_n
+            sd.put(name, rows)
 
 
 class DefaultStrategy(IStrategy):
@@ -630,15 +630,12 @@ class DefaultStrategy(IStrategy):
         self._sync_sizes()
         idx = is_duplicated.nonzero().squeeze(-1)
         n, k = self._splat_data.size, int(idx.numel())
-        rows = []
-        for bi, sd in enumerate(self._buffers()):
-            d = {}
-            for name in ("means", "sh0", "shN", "scaling_raw", "rotation_raw", "opacity_raw"):
-                t = sd.tensor(name)
-                extra = t.index_select(0, idx) if bi == 0 else torch.zeros((k,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device)
-                d[name] = torch.cat([t, extra], 0)
-            rows.append(d)
-        _rewrite_rows(self._buffers(), rows, n + k)
+
+        def rows(buffer, name, old):
+            extra = old.index_select(0, idx) if buffer == 0 else torch.zeros((k,) + tuple(old.shape[1:]), dtype=old.dtype, device=old.device)
+            return torch.cat([old, extra], 0)
+
+        _rewrite_rows(self._buffers(), n, n + k, rows)
         self._sync_sizes()
         self._grads_valid = False
 
@@ -657,27 +654,25 @@ class DefaultStrategy(IStrategy):
         if noise is None:
             noise = torch.randn((2, k, 3), dtype=torch.float32, device=sd.device)
         samples = torch.einsum("nij,nj,bnj->bni", rotmats, s_scales, noise)  # [2, k, 3]
-        rows = []
-        for bi, buf in enumerate(self._buffers()):
-            d = {}
-            for gi, name in enumerate(("means", "sh0", "shN", "scaling_raw", "rotation_raw", "opacity_raw")):
-                t = buf.tensor(name)
-                rest_rows = t.index_select(0, rest)
-                if bi > 0:
-                    new = torch.zeros((2 * k,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device)
+
+        def rows(buffer, name, old):
+            kept = old.index_select(0, rest)
+            if buffer > 0:
+                new = torch.zeros((2 * k,) + tuple(old.shape[1:]), dtype=old.dtype, device=old.device)
+            else:
+                sel = old.index_select(0, idx)
+                if name == "means":
+                    new = (sel.unsqueeze(0) + samples).reshape(-1, 3)
+                elif name == "scaling_raw":
+                    new = torch.log(s_scales / 1.6).repeat(2, 1)
+                elif name == "opacity_raw" and self._params.revised_opacity:
+                    new = torch.logit(1.0 - torch.sqrt(1.0 - torch.sigmoid(sel))).repeat(2, 1)
                 else:
-                    sel = t.index_select(0, idx)
-                    if gi == 0:
-                        new = (sel.unsqueeze(0) + samples).reshape(-1, 3)
-                    elif gi == 3:
-                        new = torch.log(s_scales / 1.6).repeat(2, 1)
-                    elif gi == 5 and self._params.revised_opacity:
-                        new = torch.logit(1.0 - torch.sqrt(1.0 - torch.sigmoid(sel))).repeat(2, 1)
-                    else:
-                        new = sel.repeat((2,) + (1,) * (sel.dim() - 1))
-                d[name] = torch.cat([rest_rows, new], 0)
-            rows.append(d)
-        _rewrite_rows(self._buffers(), rows, int(rest.numel()) + 2 * k)
+                    new = sel.repeat((2,) + (1,) * (sel.dim() - 1))
+            del old
+            return torch.cat([kept, new], 0)
+
+        _rewrite_rows(self._buffers(), sd.size, int(rest.numel()) + 2 * k, rows)
         self._sync_sizes()
         self._grads_valid = False
 
@@ -703,9 +698,7 @@ class DefaultStrategy(IStrategy):
         """default_strategy.cpp:191-219."""
         self._sync_sizes()
         keep = (~is_prune.bool()).nonzero().squeeze(-1)
-        rows = [{name: sd.tensor(name).index_select(0, keep) for name in ("means", "sh0", "shN", "scaling_raw", "rotation_raw", "opacity_raw")}
-                for sd in self._buffers()]
-        _rewrite_rows(self._buffers(), rows, int(keep.numel()))
+        _rewrite_rows(self._buffers(), self._splat_data.size, int(keep.numel()), lambda _, name, rows: rows.index_select(0, keep))
         self._sync_sizes()
         self._grads_valid = False
 
