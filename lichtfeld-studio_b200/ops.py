@@ -320,7 +320,7 @@ _INDICES = {torch.int32: 32, torch.int64: 64}
 
 
 def embedding_fwd(table, indices, scale=1.0, out_dtype=None, out=None):
-    """scale * table[indices]: [*indices.shape, width] of the table's type or float32. table [rows, width] float32, bfloat16 or
+    """scale * table[indices], with the scale as a float32: [*indices.shape, width] of the table's type or float32. table [rows, width] float32, bfloat16 or
     float16; indices int32 or int64 of any shape. An index below 0 or not below `rows` gives zeros. `out` receives the result
     (contiguous, its element type is the out_dtype; it must not overlap the inputs)."""
     _check_typed(table, "table", _DTYPES)
@@ -381,9 +381,9 @@ def embedding_sort(indices, rows):
 
 
 def embedding_bwd(v_out, order, scale=1.0, out=None, accumulate=False):
-    """Gradient of embedding_fwd with respect to the table: [rows, width] float32, scale times the sum of v_out over every row's
-    lookups, zeros for rows without any. v_out [*indices.shape, width] float32, bfloat16 or float16. `out` receives it, or is added to with
-    `accumulate` (it must not overlap v_out). The same call gives the same bits."""
+    """Gradient of embedding_fwd with respect to the table: [rows, width] float32, scale (a float32, as the lookup's) times the sum of v_out over
+    every row's lookups, as added with twice float32's bits and rounded once; zeros for rows without any. v_out [*indices.shape, width] float32, bfloat16 or float16. `out` receives it, or is added to with
+    `accumulate` (it must not overlap v_out). The same call gives the same bits on the same model of GPU."""
     if not isinstance(order, EmbeddingOrder):
         raise RuntimeError("order must come from embedding_sort")
     device, n, rows = order._buffer.device, order.n, order.rows

@@ -1,7 +1,8 @@
 """Embedding lookup, the order of its lookups, its gradient, and a palette trained with them.
 
-The lookup is one product per element rounded once to float32 and once more to the output's type: elementary torch operations give the same bits. The gradient adds
-k values in chunks of 64 and then the chunks: an error of at most (64 + chunks + 2) U of the sum of magnitudes, U = 2^-24."""
+The lookup is one product per element rounded once to float32 and once more to the output's type: elementary torch operations give the same bits. The gradient's sums have
+twice float32's bits; how exact they are is tested in test_gpu_embedding_sums.py, and the gradients here are held to what sums in float32 keep: with U = 2^-24, an error of some U for every addition of the
+sum of magnitudes."""
 import numpy as np
 import pytest
 import torch
