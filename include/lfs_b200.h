@@ -428,7 +428,8 @@ int lfs_adam_step_segments(int n_segments, const lfs_adam_segment* segments /* h
  * over the largest code (448, 57344). What is written back is rounded down or up by a threshold that depends on the element's
  * index and t only, so that a moment that changes by less than the distance of two codes still moves by the right amount over
  * the steps, and a run repeats bit for bit; a second moment above zero is not held as zero. The update itself uses the moments before
- * that rounding. eps is zero or in [2^-126, 2^126]. A block whose largest magnitude is below 2^-110 is held as zeros; a first moment that is not finite is held as NaN.
+ * that rounding. eps is zero or in [2^-126, 2^126]. A block whose largest magnitude is below 2^-110 is held as zeros; a first moment that is not finite is held as NaN,
+ * an infinite second one as infinite (the scale is that of the block's finite numbers).
  * All zeros (codes and scales) is a fresh state. Tensors must not overlap. Empty tensors (n = 0) are skipped. Pointers are aligned to their element;
  * rows of 16 bytes (4 for codes, 8 for 16-bit gradients) let whole vectors be read.
  * A captured launch repeats its own t when it is replayed. */

@@ -70,6 +70,7 @@ constexpr int kStages = 2, kCtas8 = 4, kCtas32 = 3;
 constexpr uint32_t kGolden = 0x9E3779B9u, kPlastic = 0xC13FA9A9u, kPlastic2 = 0x91E10DA5u;
 constexpr float kTopM = 448.0f, kTopV = 57344.0f;
 constexpr float kTiny = 0x1p-110f;   // below it a scale would not be a normal number; such a block is held as zeros
+constexpr float kNormal = 0x1p-126f;   // the scale of such a block if it has infinities
 
 // Two 32-bit operations to an instruction, each rounded as the single one is.
 using f32x2 = unsigned long long;
@@ -165,7 +166,7 @@ __device__ __forceinline__ uint32_t encode_block(const Block4& b, uint32_t e, ui
 #pragma unroll
         for (int k = 0; k < 4; ++k) f.x[k] = isfinite(b.x[k]) ? b.x[k] : 0.0f;
     const Scaling s = scaling<SECOND>(warp_max(max4(f)));
-    *scale = s.scale;
+    *scale = !finite && s.scale == 0.0f ? kNormal : s.scale;   // infinity times zero would not be infinite
     uint32_t codes = encode4<SECOND>(f, s.inverse, e, offset, nearest);
     if (!finite)
 #pragma unroll
