@@ -7,12 +7,13 @@
 // written back is rounded, and the update uses the moments before that rounding.
 //
 // How it is rounded decides whether 8 bits work at all. A second moment changes by 0.1 % a step and its codes are 12 to 25 % apart, so a value that
-// is rounded to the nearest code never leaves it (on gradients of changing visibility the moment settled at 1.5 times its mean, and what was rounded to zero took steps
-// thousands of times too long). Here element i of step t is rounded down, or up if its fraction of a code's distance plus a threshold reaches one:
+// is rounded to the nearest code leaves it only as far as the block's scale moves (gradients that halve beside a steady largest one: the moment stays at 4.1 times its value), and what is rounded to zero
+// takes its next steps without a denominator. Here element i of step t is rounded down, or up if its fraction of a code's distance plus a threshold reaches one:
 //   threshold_m = frac(i r1 + t r0), threshold_v = frac(i r0 + t r2), t the tensor's own step number, r0 the golden ratio's fraction, r1 and r2 those of the plastic number's powers
 // The multiples of r0 and r2 spread evenly over [0, 1) (Weyl), so over the steps every moment moves by what it should on average, and a run can be
-// repeated bit for bit. The second moment is not rounded down to zero, which would leave the next denominator without its history. Same gradients, 6000 steps:
-// second moment 0.985 of its mean, path of the parameters 11 % off (the noise of the moments), against nearest codes 1.55 and thousands.
+// repeated bit for bit. The second moment is not rounded down to zero, which would leave the next denominator without its history. 6000 steps
+// of gradients that are there in half of them and become five times smaller: second moments 0.99 of their own on average, path of the parameters 11 % off (the noise of the moments); nearest codes 1.07 to 1.6, and from
+// 20 % to thousands of times, by the numbers drawn. Beside a steady largest one: 0.985, 6 %. (tests/test_gpu_adamw_step.py)
 //
 // Explicit roundings (no contracted products), so that a code does not depend on how the compiler forms an expression.
 #include "optim.cuh"
