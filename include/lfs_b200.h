@@ -431,8 +431,10 @@ int lfs_adam_step_segments(int n_segments, const lfs_adam_segment* segments /* h
  * that rounding. eps is zero or in [2^-126, 2^126]. A block whose largest magnitude is below 2^-110 is held as zeros; a first moment that is not finite is held as NaN,
  * an infinite second one as infinite (the scale is that of the block's finite numbers).
  * All zeros (codes and scales) is a fresh state. Tensors must not overlap. Empty tensors (n = 0) are skipped. Pointers are aligned to their element;
- * rows of 16 bytes (4 for codes, 8 for 16-bit gradients) let whole vectors be read.
- * A captured launch repeats its own t when it is replayed. */
+ * where all of a tensor's arrays, codes and scales among them, begin on 16 bytes, whole vectors are read and written (one that does not: 1.8
+ * times the time with 32-bit moments, 3.5 times with 8-bit ones).
+ * A captured launch repeats its own t when it is replayed: bias corrections, and the thresholds of 8-bit moments, which then stop following slow
+ * changes. */
 #define LFS_ADAMW_BLOCK 128
 typedef struct lfs_adamw_tensor {
     float* param;
