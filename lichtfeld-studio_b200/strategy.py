@@ -257,7 +257,7 @@ class PackedMoments:
 
     def tensor(self, name: str) -> torch.Tensor:
         t = ops.adamw_state_decode(*self.live(name))
-        return t.view(self.size, -1, 3) if name in ("sh0", "shN") else t.view(self.size, self._w[name])
+        return t.view(self.size, self._w[name] // 3, 3) if name in ("sh0", "shN") else t.view(self.size, self._w[name])
 
     def put(self, name: str, rows: torch.Tensor):
         codes, scales = self.live(name)
