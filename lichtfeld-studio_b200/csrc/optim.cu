@@ -244,11 +244,25 @@ __device__ __forceinline__ float half_bits(uint32_t bits, int dtype) {
 __device__ __forceinline__ float fast_root(float x) { float r; asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float fast_reciprocal(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
+// The same rounded once. Very small operands take the approximations, since root and division of CUDA leave their short path for them: first moments of rows that have not been seen for some hundreds of steps
+// are below the normal numbers, and a step of 59 M elements then took 311 us instead of 270.
+constexpr float kShortPath = 0x1p-100f;
+__device__ __forceinline__ float root(float x) {
+    const bool tiny = x < kShortPath;
+    const float r = __fsqrt_rn(tiny ? 1.0f : x);
+    return tiny ? fast_root(x) : r;
+}
+__device__ __forceinline__ float quotient(float a, float b) {
+    const bool tiny = fabsf(a) < kShortPath;
+    const float q = __fdiv_rn(tiny ? 1.0f : a, b);
+    return tiny ? __fmul_rn(a, fast_reciprocal(b)) : q;
+}
+
 struct Step {
     float grad_scale, beta1, beta2, one_minus_beta1, one_minus_beta2, bc2_sqrt_rcp, eps, minus_zero, step_size, decay;
 };
-// FAST: the step takes the approximate root and reciprocal, off by 2^-23 of it each. With 32-bit moments both are rounded once, which is free there (59 M elements 258 us either way: memory; 400 small
-// tensors 5.5 and 6.3). With 8-bit moments, which are themselves 2^-5 and more off, they would add half to the time (177 M elements 725 us against 480 to 520, 4.6 M 27.7 against 20.7).
+// FAST: the step takes the approximate root and reciprocal, off by 2^-23 of it each. With 32-bit moments both are rounded once, which costs nothing there to 1.5 % (59 M elements 258 us either way, 266 and 270 in a
+// long run; 400 small tensors 5.5). With 8-bit moments, which are themselves 2^-5 and more off, they would add half to the time (177 M elements 725 us against 480 to 520, 4.6 M 27.7 against 20.7).
 template <bool FAST>
 __device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Block4& g, const Step& S) {
     const f32x2 zero = pair(S.minus_zero, S.minus_zero);
@@ -262,8 +276,8 @@ __device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Bl
         // The moments are rounded step by step, since their codes depend on it.
         // A denominator is zero or normal: the root of the smallest number is 2^-74.5, and an eps below 2^-126 is refused.
         const float v0 = v.x[2 * i], v2 = v.x[2 * i + 1];
-        const f32x2 root = FAST ? pair(fast_root(v0), fast_root(v2)) : pair(__fsqrt_rn(v0), __fsqrt_rn(v2));
-        const f32x2 denominator = add2(mul2(root, pair(S.bc2_sqrt_rcp, S.bc2_sqrt_rcp)), pair(S.eps, S.eps)), numerator = mul2(m1, pair(S.step_size, S.step_size));
+        const f32x2 roots = FAST ? pair(fast_root(v0), fast_root(v2)) : pair(root(v0), root(v2));
+        const f32x2 denominator = add2(mul2(roots, pair(S.bc2_sqrt_rcp, S.bc2_sqrt_rcp)), pair(S.eps, S.eps)), numerator = mul2(m1, pair(S.step_size, S.step_size));
         float a, b;
         unpair(denominator, a, b);
         f32x2 step;
@@ -272,7 +286,7 @@ __device__ __forceinline__ void update(Block4& p, Block4& m, Block4& v, const Bl
         } else {
             float c, d;
             unpair(numerator, c, d);
-            step = pair(__fdiv_rn(c, a), __fdiv_rn(d, b));
+            step = pair(quotient(c, a), quotient(d, b));
         }
         p.set(i, sub2(mul2(p.get(i), pair(S.decay, S.decay)), step));
     }

@@ -85,3 +85,26 @@ def test_8_bit_moments_fall_beside_a_steady_largest_one(pkg):
     ratio, near, off, near_off = long_run(pkg, n, steps, gradient)
     print(f"second moment {ratio[~top].mean():.3f} of its own (nearest codes {near[~top].mean():.3f}), path off by {off:.3f} (nearest codes {near_off:.3g})")
     assert abs(ratio[~top].mean() - 1) < 0.1 and off < 0.3 and near[~top].mean() > 3
+
+
+def test_rows_that_have_not_been_seen_for_long(pkg):
+    """First moments that 1500 steps without a gradient made smaller than any normal number (0.9^1500 = 2^-228), and second moments that never had one, next to rows that are seen: the former stay where they are,
+    the latter have the bits of a tensor of their own."""
+    st = pkg.strategy
+    n, seen = 4096, torch.arange(4096, device="cuda") % 2 == 0
+    gen = torch.Generator("cuda").manual_seed(2)
+    P = torch.randn(n, device="cuda", generator=gen)
+    G = torch.randn(n, device="cuda", generator=gen)
+    G[1::4] = 0.0                                   # of the rows that are not seen later, half never had a gradient
+    opt = st.AdamW([P], [G], lr=1e-3, eps=1e-15, weight_decay=0.0)
+    opt.step()
+    G[~seen] = 0.0
+    for _ in range(1500):
+        opt.step()
+    m = opt.moments[0].exp_avg
+    assert m[3::4].abs().max() < 2.0 ** -126 and m[1::4].eq(0).all() and opt.moments[0].exp_avg_sq[1::4].eq(0).all()
+    one = st.AdamW([P[seen].clone()], [G[seen].clone()], lr=1e-3, eps=1e-15, weight_decay=0.0, moments=[st.Moments(m[seen].clone(), opt.moments[0].exp_avg_sq[seen].clone())])
+    one.step_count = opt.step_count
+    before = P.clone()
+    opt.step(), one.step()
+    assert torch.equal(P[~seen], before[~seen]) and torch.equal(P[seen], one.params[0])
