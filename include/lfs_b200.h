@@ -475,11 +475,11 @@ int lfs_embedding_sort(int64_t n, int64_t rows, const void* indices, int index_b
  * v_out[i] (v_out [n,width] of type `dtype`), zeros for rows without lookups; added to v_table with `accumulate`. order and sorted_rows are those of
  * lfs_embedding_sort for the same n and rows, 16-byte aligned. Sums are held in two floats each, so the result is that of sums with
  * twice float32's bits, rounded once: off by 2^-24 of itself, and for a row of k lookups by at most 6 k^2 2^-48 of scale times the sum of
- * their magnitudes (which shows only where large addends cancel). scale is the lookup's float32. The same call gives the same
+ * their magnitudes (which shows only where large addends cancel). The scale counts with 48 bits. The same call gives the same
  * bits on the same model of GPU (the lookups are cut by its SMs). */
 size_t lfs_embedding_bwd_workspace_bytes(int64_t n, int width);
 int lfs_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order,
-                      const int32_t* sorted_rows, float scale, int accumulate, float* v_table, void* workspace,
+                      const int32_t* sorted_rows, double scale, int accumulate, float* v_table, void* workspace,
                       size_t workspace_bytes, void* stream);
 
 /* Data-parallel exchange fused with the optimizer (no counterpart in the reference, which is single-GPU):

@@ -125,7 +125,7 @@ _SIGNATURES = {
     "lfs_adamw_state_decode": [i64, vp, vp, i32, vp, vp],
     "lfs_embedding_fwd": [i64, i64, i32, vp, i32, vp, i32, f32, vp, i32, vp],
     "lfs_embedding_sort": [i64, i64, vp, i32, vp, vp, vp, sz, vp],
-    "lfs_embedding_bwd": [i64, i64, i32, vp, i32, vp, vp, f32, i32, vp, vp, sz, vp],
+    "lfs_embedding_bwd": [i64, i64, i32, vp, i32, vp, vp, C.c_double, i32, vp, vp, sz, vp],
     "lfs_dp_reduce_adam_broadcast": [i32, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), vp, i32, C.POINTER(DpSegment), C.c_double,
                                      C.c_double, C.c_double, i64, f32, i32, vp],
     "lfs_dp_signal": [i32, C.POINTER(C.c_void_p), i32, i32, i32, vp],

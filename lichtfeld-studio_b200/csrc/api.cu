@@ -1094,7 +1094,7 @@ size_t lfs_embedding_bwd_workspace_bytes(int64_t n, int width) {
     return embedding_bwd_bytes(n, width);
 }
 
-int lfs_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, float scale,
+int lfs_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, double scale,
                       int accumulate, float* v_table, void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = check_embedding("lfs_embedding_bwd", n, rows, width);
     if (rc != LFS_OK) return rc;

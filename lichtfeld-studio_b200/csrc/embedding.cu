@@ -6,6 +6,8 @@
 // keep it over many steps.
 #include "embedding.cuh"
 
+#include <cmath>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -412,6 +414,13 @@ constexpr int64_t kOwnClear = 32768;   // elements of a table that a single CTA 
 // CTAs per SM by the sums that a lane holds
 constexpr int bwd_ctas(int sums) { return sums <= 4 ? 3 : 2; }
 
+// A number in two floats. The lookup's scale is a float32, as its products are; here the sums have more bits than that.
+struct Scale { float hi, lo; };
+Scale two_floats(double x) {
+    const float hi = (float)x;
+    return {hi, std::isfinite(hi) ? (float)(x - hi) : 0.0f};
+}
+
 // A sum in two floats: every rounding of the first is exact in the second (Knuth's two-sum). Explicit roundings, so that none of it is simplified away.
 struct Sum {
     float hi, lo;
@@ -424,15 +433,17 @@ struct Sum {
         add(o.hi);
         lo = __fadd_rn(lo, o.lo);
     }
+    // what the product of the first floats leaves of the sum times scale
+    __device__ __forceinline__ float rest(Scale scale, float p) const { return __fmaf_rn(lo, scale.hi, __fmaf_rn(hi, scale.lo, __fmaf_rn(hi, scale.hi, -p))); }
     // the sum times scale, rounded once; once it is infinite or NaN the roundings say nothing
-    __device__ __forceinline__ float times(float scale) const {
-        const float p = __fmul_rn(hi, scale);
-        return isfinite(p) ? __fadd_rn(p, __fmaf_rn(lo, scale, __fmaf_rn(hi, scale, -p))) : p;
+    __device__ __forceinline__ float times(Scale scale) const {
+        const float p = __fmul_rn(hi, scale.hi);
+        return isfinite(p) ? __fadd_rn(p, rest(scale, p)) : p;
     }
     // and added to `more`
-    __device__ __forceinline__ float times(float scale, float more) const {
-        const float p = __fmul_rn(hi, scale);
-        Sum r{more, __fmaf_rn(lo, scale, __fmaf_rn(hi, scale, -p))};
+    __device__ __forceinline__ float times(Scale scale, float more) const {
+        const float p = __fmul_rn(hi, scale.hi);
+        Sum r{more, rest(scale, p)};
         r.add(p);
         return isfinite(r.hi) ? __fadd_rn(r.hi, r.lo) : r.hi;
     }
@@ -467,7 +478,7 @@ struct Sums {
 
 template <int DTYPE, int V, int C, int T>
 __global__ void __launch_bounds__(kBwdThreads, bwd_ctas(C * V)) embedding_bwd_kernel(int64_t n, int64_t rows, int width, int log_group, int share, int clear, const typename Element<DTYPE>::T* __restrict__ v_out,
-                                                                    const int32_t* __restrict__ order, const int32_t* __restrict__ sorted_rows, float scale, int accumulate,
+                                                                    const int32_t* __restrict__ order, const int32_t* __restrict__ sorted_rows, Scale scale, int accumulate,
                                                                     float* __restrict__ v_table, Sum* __restrict__ parts) {
     using In = Pack<DTYPE, V>;
     __shared__ __align__(16) int32_t row_s[4 * kBwdThreads], at_s[4 * kBwdThreads];
@@ -629,7 +640,7 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_ctas(C * V)) embedding_bwd_ke
 // The rows that lie in several stretches: the one that has a row's tail adds the heads of those that follow. A CTA per stretch; its threads are columns by slices of the heads.
 constexpr int kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int64_t n, int64_t rows, int width, int stretch, int stretches, const int32_t* __restrict__ sorted_rows,
-                                                                      float scale, int accumulate, const Sum* __restrict__ parts, float* __restrict__ v_table) {
+                                                                      Scale scale, int accumulate, const Sum* __restrict__ parts, float* __restrict__ v_table) {
     __shared__ Sum sum_s[kJoinThreads];
     __shared__ int next_s;
     wait_for_previous();
@@ -684,7 +695,7 @@ struct Bwd {
     int width, log_group, accumulate;
     const void* v_out;
     const int32_t *order, *sorted_rows;
-    float scale;
+    Scale scale;
     float* v_table;
     Sum* parts;
     cudaStream_t st;
@@ -779,7 +790,7 @@ int launch_embedding_sort(int64_t n, int64_t rows, const void* indices, int inde
 
 size_t embedding_bwd_bytes(int64_t n, int width) { return bwd_stretches(n) <= 1 ? 0 : (size_t)bwd_stretches(n) * 2 * width * sizeof(Sum); }
 
-int launch_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, float scale,
+int launch_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, double scale,
                          int accumulate, float* v_table, void* workspace, cudaStream_t st) {
     LFS_TIMED("embedding_bwd", st);
     if (n == 0) {
@@ -789,7 +800,7 @@ int launch_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, 
         }
         return LFS_OK;
     }
-    const Bwd b{n, rows, width, 0, accumulate, v_out, order, sorted_rows, scale, v_table, static_cast<Sum*>(workspace), st};
+    const Bwd b{n, rows, width, 0, accumulate, v_out, order, sorted_rows, two_floats(scale), v_table, static_cast<Sum*>(workspace), st};
     return dtype == LFS_F32 ? bwd_type<LFS_F32>(b) : dtype == LFS_BF16 ? bwd_type<LFS_BF16>(b) : bwd_type<LFS_F16>(b);
 }
 

@@ -12,7 +12,7 @@ size_t embedding_sort_bytes(int64_t n, int64_t rows);
 int launch_embedding_sort(int64_t n, int64_t rows, const void* indices, int index_bits, int32_t* order, int32_t* sorted_rows, void* workspace, cudaStream_t st);
 
 size_t embedding_bwd_bytes(int64_t n, int width);
-int launch_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, float scale,
+int launch_embedding_bwd(int64_t n, int64_t rows, int width, const void* v_out, int dtype, const int32_t* order, const int32_t* sorted_rows, double scale,
                          int accumulate, float* v_table, void* workspace, cudaStream_t st);
 
 }  // namespace lfs

@@ -381,8 +381,8 @@ def embedding_sort(indices, rows):
 
 
 def embedding_bwd(v_out, order, scale=1.0, out=None, accumulate=False):
-    """Gradient of embedding_fwd with respect to the table: [rows, width] float32, scale (a float32, as the lookup's) times the sum of v_out over
-    every row's lookups, as added with twice float32's bits and rounded once; zeros for rows without any. v_out [*indices.shape, width] float32, bfloat16 or float16. `out` receives it, or is added to with
+    """Gradient of embedding_fwd with respect to the table: [rows, width] float32, scale times the sum of v_out over every row's
+    lookups, as added with twice float32's bits and rounded once; zeros for rows without any. v_out [*indices.shape, width] float32, bfloat16 or float16. `out` receives it, or is added to with
     `accumulate` (it must not overlap v_out). The same call gives the same bits on the same model of GPU."""
     if not isinstance(order, EmbeddingOrder):
         raise RuntimeError("order must come from embedding_sort")

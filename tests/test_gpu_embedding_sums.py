@@ -2,10 +2,10 @@
 
 A row's sum is held in two floats: every addition to the first is followed by what it rounded off (Knuth's two-sum, exact), which is added to the second in float32. With U = 2^-24, S the sum of
 the magnitudes of a row's addends and K the most additions that one of them goes through, the roundings that the second float gathers are at most K U S together, and D additions in float32 lose
-at most D U of that: D K U^2 S. The result (first + second) * scale is then rounded once, and its products lose U^2 (K + 2) S more.
+at most D U of that: D K U^2 S. The result (first + second) * scale is then rounded once, and its products lose U^2 (K + 3) S more (the scale is in two floats as well).
 
 Here n <= 20,011: a group of lanes adds at most 128 lookups one after the other, its sum is joined with those of at most 128 groups by halves (7) and of one neighbour (1), and the stretches, at
-most 20 of 1,024 lookups, one after the other: K <= 156. A join adds to the second float twice: D <= 128 + 2 * 28 = 184. D K + K + 2 < 3e4. With `accumulate` one more addition of the same kind, whose
+most 20 of 1,024 lookups, one after the other: K <= 156. A join adds to the second float twice: D <= 128 + 2 * 28 = 184. D K + K + 3 < 3e4. With `accumulate` one more addition of the same kind, whose
 addend is the old value. So the result is off by U of itself and 3e4 U^2 = 0.0018 U of the magnitudes' sum; sums in plain float32 are off by hundreds of U of the magnitudes' sum here."""
 import numpy as np
 import pytest
@@ -68,13 +68,12 @@ def test_sums_are_those_of_twice_the_bits(pkg, dtype, width):
             for offset in (0, 1):
                 v = gradients(n, width, DTYPES[dtype], kind, n + width, offset)
                 for scale in (1.0, 1.7):
-                    scale32 = float(np.float32(scale))      # the scale is a float32, as the lookup's
                     got = ops.embedding_bwd(v, order, scale)
-                    want, size = sums(v, index, rows, scale32)
+                    want, size = sums(v, index, rows, scale)
                     assert ((got.double() - want).abs() <= allowed(want, size)).all(), (n, kind, offset, scale)
                     base = torch.randn(rows, width, generator=torch.Generator().manual_seed(3)).cuda()
                     added = ops.embedding_bwd(v, order, scale, out=base.clone(), accumulate=True)
-                    want, size = sums(v, index, rows, scale32, base)
+                    want, size = sums(v, index, rows, scale, base)
                     assert ((added.double() - want).abs() <= allowed(want, size)).all(), (n, kind, offset, scale, "accumulate")
                     assert torch.equal(got, ops.embedding_bwd(v, order, scale))
 
@@ -91,3 +90,19 @@ def test_large_gradients_that_cancel(pkg, big):
         assert ((got.double() - want).abs() <= allowed(want, size)).all()
         # of the two floats the first alone would be off by the last place of B: 2^-24 B for every lookup
         assert ((got.double() - want).abs().max() < U * big)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("scale", [1.0, 1.7, -0.3, 0.5 * 45 ** 0.5, 1e-3, 2.0 ** 40 / 3])
+def test_scale_and_sum_are_rounded_once(pkg, dtype, scale):
+    """Rows of one to four lookups against the product of their exact sum with the scale as given: half a last place, and 2^-10 of one for what two floats cut off (2^-48 of sum and scale each, against a last
+    place of 2^-24 at the least)."""
+    ops = pkg.ops
+    n, rows = 5000, 2000
+    index = torch.cat([torch.arange(rows), torch.randint(rows, (n - rows,), generator=torch.Generator().manual_seed(1))]).to(torch.int32).cuda()
+    v = gradients(n, 45, DTYPES[dtype], "normal", 2, 0)
+    v.abs_()                                     # nothing cancels
+    got = ops.embedding_bwd(v, ops.embedding_sort(index, rows), scale).cpu().numpy()
+    want = sums(v, index, rows, scale)[0].cpu().numpy()
+    place = np.spacing(np.abs(want).astype(np.float32)).astype(np.float64)
+    assert (np.abs(got - want) <= (0.5 + 2.0 ** -10) * place).all()
