@@ -356,7 +356,7 @@ static_assert(kThreads * 4 == kRow && kTile % (8 * kThreads) == 0, "whole copies
 
 // Moments in 8 bits. Issue slots and memory are both near their limits (65 instructions for 16 bytes; 66 % of both), so the copies are wide and asynchronous: loads straight into registers wait for one another at every
 // block and cost more instructions for their addresses. us for 3 M Gaussians at SH degree 3 (177 M elements): simple 1018, codes from scaled bits 755, the next block's loads under way 592, tiles copied
-// ahead 515, one division and one check for both moments 459 (96 % of the copy rate). In a long run, where the clock is lower, 503 (88 %).
+// ahead 515, one division and one check for both moments 459 to 510 by the GPU and the run (86 to 96 % of the copy rate). In a long run, where the clock is lower, 503 to 534 (82 to 88 %).
 template <int CAP>
 __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
     extern __shared__ __align__(128) char stages_s[];
@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(kThreads, kCtas8) adamw8_kernel(const __grid_c
     }
 }
 
-// Moments in 32 bits: nothing but memory. A tile is a block to a warp, and the next one's loads are under way while it is computed: 59 M elements 258 us, 99 % of the copy rate (simple 321).
+// Moments in 32 bits: memory. A tile is a block to a warp, and the next one's loads are under way while it is computed: 59 M elements 258 us, 99 % of the copy rate (simple 321); 270 to 281 in a long run, of which
+// 2 % are the root and the division.
 template <int CAP>
 __global__ void __launch_bounds__(kThreads, kCtas32) adamw32_kernel(const __grid_constant__ AdamWArgs<CAP> A) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x;
