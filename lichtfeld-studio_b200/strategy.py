@@ -164,13 +164,23 @@ class AdamW:
         self.lr, self.weight_decay = lr, weight_decay
         self.step_count = 0
         self._table, self._rates = np.zeros(n, _TABLE), None
-        self.missed = self._table["missed"]
         self._address = self._table.ctypes.data
         self._table["param"] = [p.data_ptr() for p in self.params]
         for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
             self._table[name] = [0 if getattr(m, name) is None else getattr(m, name).data_ptr() for m in self.moments]
         self._check_written([p.numel() for p in self.params])
         self.set_grads(grads)
+
+    @property
+    def missed(self) -> np.ndarray:
+        return self._table["missed"]
+
+    @missed.setter
+    def missed(self, value):
+        counts = np.asarray(value, dtype=np.int64)
+        if counts.shape != (len(self.params),) or (counts < 0).any() or (counts >= 1 << 31).any():
+            raise RuntimeError(f"missed: one count for each of {len(self.params)} tensors, got {value}")
+        self._table["missed"] = counts
 
     @property
     def lr(self) -> list:

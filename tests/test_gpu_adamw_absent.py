@@ -70,3 +70,30 @@ def test_tensors_that_come_and_go(st, bits):
     for i in range(len(sizes)):
         assert 7 - opt.missed[i] == alone[i].step_count
         assert all(torch.equal(a, b) for a, b in zip(state(opt, i), state(alone[i], 0))), i
+
+
+def test_missed_is_set_like_step_count(pkg, st):
+    """Setting the counts sets what the steps go by, from a list or from another optimizer's, which stay apart from then on."""
+    def make():
+        return st.AdamW([values(40, 1), values(50, 2)], [values(40, 3), values(50, 4)], lr=1e-2)
+    a, b = make(), make()
+    a.step_count, a.missed = 10, [0, 7]
+    b.step_count, b.missed = 10, a.missed
+    a.set_grads([a.grads[0], None])
+    a.step()
+    assert a.missed.tolist() == [0, 8] and b.missed.tolist() == [0, 7]
+    b.step()
+    one = st.AdamW([values(50, 2)], [values(50, 4)], lr=1e-2)
+    one.step_count = 3
+    one.step()
+    assert torch.equal(b.params[1], one.params[0]) and torch.equal(a.params[0], b.params[0]) and torch.equal(a.params[1], values(50, 2))
+    for bad in ([1], [0, -1], 3, [0, 1 << 31], [[0, 0]]):
+        with pytest.raises(RuntimeError, match="missed"):
+            b.missed = bad
+    assert b.missed.tolist() == [0, 7]
+    b.missed[:] = 11                      # as many as there were steps: the next one is the first
+    b.step()
+    b.missed[1] = 13
+    with pytest.raises(Exception, match="missed"):
+        b.step()
+    assert b.step_count == 12
