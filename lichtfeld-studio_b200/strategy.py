@@ -332,7 +332,7 @@ def make_optimizer(model: SplatData, lrs, params) -> FusedAdam:
         return FusedAdamW(model, lrs, (0.9, 0.999), 1e-15, decay, bits)
     if kind != "adam":
         raise RuntimeError(f"optimizer must be adam or adamw, got {kind}")
-    if bits != 32 or (decay if isinstance(decay, (int, float)) else any(decay)):
+    if bits != 32 or (decay if isinstance(decay, numbers.Real) else any(decay)):
         raise RuntimeError("weight_decay and state_bits need optimizer=\"adamw\"")
     return FusedAdam(model, lrs, (0.9, 0.999), 1e-15)
 

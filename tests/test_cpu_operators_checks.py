@@ -52,6 +52,19 @@ def test_gradients_of_another_scene_are_refused(pkg):
         assert grads.size == size and opt.step_count == 0
 
 
+def test_weight_decay_may_be_any_number(pkg):
+    """numpy's scalars too, as one value for all groups."""
+    import numpy as np
+    st = pkg.strategy
+    model = pkg.trainer.SplatData(10, 4, torch.device("cpu"))
+    for zero in (0, 0.0, np.float32(0), np.float64(0)):
+        assert type(st.make_optimizer(model, [1e-3] * 6, st.OptimizationParameters(weight_decay=zero))) is st.FusedAdam
+    for some in (1, 0.5, np.float32(0.5), np.float64(0.5)):
+        assert st.make_optimizer(model, [1e-3] * 6, st.OptimizationParameters(optimizer="adamw", weight_decay=some)).weight_decay == [float(some)] * 6
+        with pytest.raises(RuntimeError, match="adamw"):
+            st.make_optimizer(model, [1e-3] * 6, st.OptimizationParameters(weight_decay=some))
+
+
 # ---- checkpoints ----------------------------------------------------------------------------------------------------
 def strategy(pkg, kind="MCMC", **kw):
     st, tr = pkg.strategy, pkg.trainer
